@@ -1,7 +1,7 @@
 /* libmbvae_hip.so -- C ABI of the MI355X (gfx950) kernels behind the MB-VAE-DTI hot path.
  *
  * Conventions (all entry points):
- *   - every pointer is a DEVICE pointer (fp32 unless noted; masks are uint8, class ids int64);
+ *   - every pointer is a DEVICE pointer unless noted (fp32 unless noted; masks are uint8, class ids int64);
  *     tensors are dense row-major with the feature dimension contiguous;
  *   - nothing is allocated, freed or synchronised: outputs and workspaces are caller-owned, work is
  *     enqueued on `stream` and the call returns immediately;
@@ -138,6 +138,31 @@ int mbvae_gate_fwd(const float* x, const float* u, const float* z, const uint8_t
                    mbvae_stream_t stream);
 int mbvae_gate_bwd(const float* dy, const float* u, const float* z, const uint8_t* keep, float scale, float* du, float* dz,
                    int64_t n, int u_is_x, mbvae_stream_t stream);
+
+/* ---- Gated residual update between two norms ---------------------------------------------------------------
+ * What every residual block of the encoders does around its products (models/blocks.py:125 `x + x * att(x)`, :127 `x + mlp(x)`,
+ * :318-328, and the LayerNorm that opens the next block), as one kernel each way:
+ *   v = N_post(u);   y = x + scale * w * v;   n = N_pre(y);   w = sigmoid(z) * (keep ? keep_scale : 0)
+ * u == NULL: u is x.  z == NULL: no gate.  keep (uint8 [rows, D], contiguous) == NULL: nothing is dropped; where keep is 0 nothing is
+ * added, whatever v and z hold there.  scale, gammas, betas: [D] of type ptype; post_gamma == NULL / pre_gamma == NULL: that norm is
+ * absent (n is then not written); a beta may be NULL.  rms: root-mean-square norms, no mean is taken out.  x, u, z, dy, dn: rows ld*
+ * elements apart, elements of a row contiguous, any alignment; outputs contiguous.  dtype / ptype: 0 fp32, 1 bf16, 2 fp16; all
+ * arithmetic is fp32.  1 <= D <= 8192, rows < 2^31.  stats (float [rows, 4], 16-byte aligned): written by the forward for the
+ * backward, NULL where there is none.
+ * Backward: dy / dn NULL: that output has no gradient.  du only where u was given, dz only where z was; any output may be NULL; with
+ * u == NULL dx is the whole gradient of x.  dscale ... dpre_beta: [D] of type ptype, overwritten.  workspace: at least
+ * mbvae_gated_norm_bwd_workspace(rows, D, dtype) bytes, 16-byte aligned.  Bitwise reproducible. */
+int mbvae_gated_norm_fwd(const void* x, int64_t ldx, const void* u, int64_t ldu, const void* z, int64_t ldz, const uint8_t* keep,
+                         float keep_scale, const void* post_gamma, const void* post_beta, const void* scale,
+                         const void* pre_gamma, const void* pre_beta, void* y, void* n, float* stats, int64_t rows, int64_t D,
+                         int rms, float eps, int dtype, int ptype, mbvae_stream_t stream);
+int64_t mbvae_gated_norm_bwd_workspace(int64_t rows, int64_t D, int dtype);
+int mbvae_gated_norm_bwd(const void* x, int64_t ldx, const void* u, int64_t ldu, const void* z, int64_t ldz, const uint8_t* keep,
+                         float keep_scale, const void* post_gamma, const void* post_beta, const void* scale,
+                         const void* pre_gamma, const float* stats, const void* dy, int64_t lddy, const void* dn, int64_t lddn,
+                         void* dx, void* du, void* dz, void* dscale, void* dpost_gamma, void* dpost_beta, void* dpre_gamma,
+                         void* dpre_beta, int64_t rows, int64_t D, int rms, float eps, int dtype, int ptype, void* workspace,
+                         int64_t ws_bytes, mbvae_stream_t stream);
 
 /* ---- Edge-feature attention ------------------------------------------------------------------------
  * Replaces graph_transformer.py:206-249 (Y = Q*K/sqrt(df); Y*(E1+1)+E2; FiLM by y; per-channel masked
@@ -397,6 +422,32 @@ int mbvae_linear_bwd_weight_bf16(const void* dy, int dy_bf16, int64_t lddy, cons
  * bs*n*(n+1) bytes instead of the one-hot floats. */
 int mbvae_dense_from_ids(const int8_t* atoms, const int8_t* bonds, float* X, float* E, uint8_t* mask, int64_t bs,
                          int64_t n, int64_t cx, int64_t ce, mbvae_stream_t stream);
+
+/* ---- Embedding lookup and its gradient ---------------------------------------------------------------------
+ * Rows of a table by class id, in place of a product with one-hot rows (graph_transformer.py:321-326 applied to the one-hot atoms
+ * and bonds of diffusion/utils.py:90-120): y[r] = scale * weight[ids[r]], weight [vocab, D], y [rows, D], both contiguous, of one type
+ * (0 fp32, 1 bf16, 2 fp16).  id_type: 1 int8, 2 int16, 3 uint8, 4 int32, 8 int64.  Ids outside [0, vocab) - the -1 of padding -
+ * give a row of zeros and take no gradient; nothing is read for them.
+ * Backward: dweight[v] = scale * sum of dy[r] over the rows with ids[r] == v, zero where there are none; dy has rows ldy elements
+ * apart.  Sums in fp32, in an order that the ids alone decide: bitwise reproducible.  workspace: at least
+ * mbvae_embedding_bwd_workspace(rows, vocab, D) bytes, 16-byte aligned.  rows, vocab < 2^31, D <= 2^23. */
+int mbvae_embedding_fwd(const void* ids, int id_type, const void* weight, void* y, int64_t rows, int64_t vocab, int64_t D,
+                        float scale, int dtype, mbvae_stream_t stream);
+int64_t mbvae_embedding_bwd_workspace(int64_t rows, int64_t vocab, int64_t D);
+int mbvae_embedding_bwd(const void* ids, int id_type, const void* dy, int64_t ldy, void* dweight, int64_t rows, int64_t vocab,
+                        int64_t D, float scale, int dtype, void* workspace, int64_t ws_bytes, mbvae_stream_t stream);
+
+/* ---- Global gradient norm and clipping ---------------------------------------------------------------------
+ * What Lightning's gradient_clip_val does between backward and the optimiser step (pl.Trainer, mb_vae_dti/training/run.py:638-654):
+ *   norm = (sum |g|^p)^(1/p) over all values of all tensors (p = 1, 2 or infinity),   dst = src * min(1, max_norm / (norm + 1e-6)).
+ * src, dst, numel, dtype are HOST arrays of `count` entries (device pointers, value counts, types 0 fp32 / 1 bf16 / 2 fp16), read
+ * before the call returns; norm is one device float.  dst == NULL: the norm alone.  dst[i] == src[i] for all i: in place (nothing is
+ * written where the norm is within max_norm).  An output may not share memory with another output, nor with an input other than
+ * its own exact place: -1.  A norm of infinity scales by 0, a NaN norm makes every gradient NaN.  workspace: at least
+ * mbvae_grad_clip_workspace(count) bytes, 8-byte aligned.  Partial sums are fp64 in a fixed order: bitwise reproducible. */
+int64_t mbvae_grad_clip_workspace(int64_t count);
+int mbvae_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int64_t count, double p,
+                    double max_norm, float* norm, void* workspace, int64_t ws_bytes, mbvae_stream_t stream);
 
 /* ---- k-cycle counts (n <= 64) ----------------------------------------------------------------------------
  * Replaces KNodeCycles.k_cycles (k3/k4/k5/k6_cycle), mb_vae_dti/training/diffusion/augmentation.py:177-250: five

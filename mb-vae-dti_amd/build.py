@@ -7,7 +7,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmbvae_hip.so")
-SOURCES = ["gemm.hip", "edge_attn.hip", "edge_fused.hip", "rowops.hip", "loss.hip", "diffusion.hip", "eigen.hip", "cycles.hip"]
+SOURCES = ["gemm.hip", "edge_attn.hip", "edge_fused.hip", "rowops.hip", "loss.hip", "diffusion.hip", "eigen.hip", "cycles.hip",
+           "gated_norm.hip", "embedding.hip", "gradclip.hip"]
 # No packed-fp32 instructions (v_pk_*_f32) in device code.  Measured on MI355X: the node-path LayerNorm backward
 # (ln_res_bwd_kernel<64, 1>), whose compiled form reads its per-row statistics through op_sel'ed packed operands, returned
 # rare wrong rows (the low half of one packed subtract behaving as "minus 0" in lanes 48-63) whenever tall-skinny product
@@ -30,7 +31,7 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    common = [os.path.join(CSRC, "common.h")]
+    common = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "typed.h")]
     jobs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)

@@ -5,7 +5,7 @@ entry point returns a non-zero status, a RuntimeError is raised.
 """
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # MBVAE_LIB selects another build of the same library (kernel A/B timing); the default is the in-tree build.
@@ -65,10 +65,20 @@ SIGNATURES = {
     "mbvae_kl_reparam_bwd": [_P, _P, _P, _P, _P, _P, _P, _L, _P],
     "mbvae_sym_eig": [_P, _P, _P, _L, _L, _P],
     "mbvae_dense_from_ids": [_P] * 5 + [_L, _L, _L, _L, _P],
+    "mbvae_gated_norm_fwd": [_P, _L, _P, _L, _P, _L, _P, _F] + [_P] * 8 + [_L, _L, _I, _F, _I, _I, _P],
+    "mbvae_gated_norm_bwd_workspace": [_L, _L, _I],
+    "mbvae_gated_norm_bwd": [_P, _L, _P, _L, _P, _L, _P, _F] + [_P] * 5 + [_P, _L, _P, _L] + [_P] * 8
+                            + [_L, _L, _I, _F, _I, _I, _P, _L, _P],
+    "mbvae_embedding_fwd": [_P, _I, _P, _P, _L, _L, _L, _F, _I, _P],
+    "mbvae_embedding_bwd_workspace": [_L, _L, _L],
+    "mbvae_embedding_bwd": [_P, _I, _P, _L, _P, _L, _L, _L, _F, _I, _P, _L, _P],
+    "mbvae_grad_clip_workspace": [_L],
+    "mbvae_grad_clip": [_P, _P, _P, _P, _L, c_double, c_double, _P, _P, _L, _P],
     "mbvae_apply_noise": [_P] * 12 + [_L, _L, _L, _L, _P],
     "mbvae_reverse_sample": [_P] * 18 + [_L, _L, _L, _L, _P],
 }
-_RET64 = {"mbvae_edge_attn_bwd_workspace", "mbvae_ln_residual_bwd_workspace", "mbvae_masked_ce_workspace", "mbvae_kl_workspace"}
+_RET64 = {"mbvae_edge_attn_bwd_workspace", "mbvae_ln_residual_bwd_workspace", "mbvae_masked_ce_workspace", "mbvae_kl_workspace",
+          "mbvae_gated_norm_bwd_workspace", "mbvae_embedding_bwd_workspace", "mbvae_grad_clip_workspace"}
 
 _STATUS = {-1: "invalid argument", -2: "unsupported shape", -3: "kernel launch failure"}
 _lib = None

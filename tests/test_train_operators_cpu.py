@@ -1,0 +1,110 @@
+"""Refusals of the embedding, gated residual norm and gradient clipping operators that the host decides on, without a GPU: the Python
+entry points on CPU tensors, and the C entry points on arguments that must never reach a launch."""
+import array
+import math
+
+import pytest
+import torch
+
+from mbvae_amd import _lib, ops
+
+EINVAL, EUNSUPPORTED = -1, -2
+A = 0x10000          # stands for a device address: a refused call never looks behind it
+
+
+def test_python_entry_points_refuse_cpu_tensors():
+    w = torch.zeros(5, 8)
+    with pytest.raises(RuntimeError, match="no CPU"):
+        ops.embedding(torch.zeros(3, dtype=torch.int64), w)
+    with pytest.raises(RuntimeError, match="no CPU"):
+        ops.gated_residual_norm(torch.zeros(3, 8))
+    with pytest.raises(RuntimeError, match="no CPU"):
+        ops.clip_grad_norm_([w], 1.0)
+    with pytest.raises(RuntimeError, match="no CPU"):
+        ops.global_grad_norm([w])
+
+
+def test_clip_argument_checks():
+    g = [torch.zeros(3)]
+    with pytest.raises(ValueError, match="outputs"):
+        ops.clip_grad_norm_(g, 1.0, out=[])
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            ops.clip_grad_norm_(g, bad)
+    for bad in (3.0, 0.5, -math.inf, math.nan):
+        with pytest.raises(ValueError, match="norm_type"):
+            ops.global_grad_norm(g, bad)
+    with pytest.raises(ValueError, match="missing"):
+        ops.clip_grad_norm_(g, 1.0, out=[None])
+
+
+def _clip(src, dst, numel, types, p=2.0, max_norm=1.0, norm=A, ws=A, ws_bytes=None):
+    lib = _lib.load()
+    n = len(src)
+    arrays = [array.array("Q", src), None if dst is None else array.array("Q", dst), array.array("q", numel), array.array("i", types)]
+    at = [0 if a is None else a.buffer_info()[0] for a in arrays]
+    return lib.mbvae_grad_clip(*at, n, p, max_norm, norm, ws, lib.mbvae_grad_clip_workspace(n) if ws_bytes is None else ws_bytes, 0)
+
+
+def test_clip_entry_refuses_before_any_launch():
+    two = dict(numel=[100, 100], types=[0, 0])
+    assert _clip([A, A], [A, A], **two) == EINVAL                       # the same tensor twice, in place
+    assert _clip([A, A + 400], [A, A + 396], **two) == EINVAL           # an output over another tensor's last value
+    assert _clip([A, A + 4000], [A + 4, A + 4000], **two) == EINVAL     # an output over its own input, shifted
+    assert _clip([A, A + 4000], [A + 8000, A + 8200], **two) == EINVAL  # outputs over each other
+    assert _clip([A, A + 4000], [A + 4000, A + 8000], **two) == EINVAL  # an output in place of another input
+    assert _clip([A + 1], [A + 1], [4], [0]) == EINVAL                  # a float at an odd address
+    assert _clip([0], None, [4], [0]) == EINVAL
+    assert _clip([A], [0], [4], [0]) == EINVAL
+    assert _clip([A], None, [-1], [0]) == EINVAL
+    assert _clip([A], None, [4], [3]) == EINVAL
+    assert _clip([A], None, [4], [0], p=3.0) == EUNSUPPORTED
+    assert _clip([A], [A], [4], [0], max_norm=-1.0) == EINVAL
+    assert _clip([A], [A], [4], [0], max_norm=math.nan) == EINVAL
+    assert _clip([A], None, [4], [0], norm=0) == EINVAL
+    assert _clip([A], None, [4], [0], ws=0) == EINVAL
+    assert _clip([A], None, [4], [0], ws=A + 4) == EINVAL
+    assert _clip([A], None, [4], [0], ws_bytes=8) == EINVAL
+
+
+def test_embedding_entries_refuse_before_any_launch():
+    lib = _lib.load()
+
+    def fwd(ids=A, id_type=8, w=A, y=A, rows=4, vocab=5, D=8, dtype=0):
+        return lib.mbvae_embedding_fwd(ids, id_type, w, y, rows, vocab, D, 1.0, dtype, 0)
+
+    def bwd(ids=A, id_type=8, dy=A, ldy=8, dw=A, rows=4, vocab=5, D=8, dtype=0, ws=A, ws_bytes=1 << 20):
+        return lib.mbvae_embedding_bwd(ids, id_type, dy, ldy, dw, rows, vocab, D, 1.0, dtype, ws, ws_bytes, 0)
+
+    for call in (fwd, bwd):
+        assert call(rows=-1) == EINVAL and call(vocab=-1) == EINVAL and call(D=-1) == EINVAL
+        assert call(id_type=5) == EINVAL and call(dtype=3) == EINVAL and call(ids=0) == EINVAL
+        assert call(rows=1 << 31) == EUNSUPPORTED and call(vocab=1 << 31) == EUNSUPPORTED and call(D=(1 << 23) + 1) == EUNSUPPORTED
+    assert fwd(w=0) == EINVAL and fwd(y=0) == EINVAL
+    assert fwd(rows=0, ids=0, y=0) == 0 and fwd(D=0) == 0
+    assert bwd(dy=0) == EINVAL and bwd(dw=0) == EINVAL and bwd(ldy=-1) == EINVAL
+    assert bwd(ws=0) == EINVAL and bwd(ws=A + 8) == EINVAL
+    assert bwd(ws_bytes=lib.mbvae_embedding_bwd_workspace(4, 5, 8) - 1) == EINVAL
+    assert bwd(vocab=0) == 0 and bwd(D=0) == 0
+
+
+def test_gated_norm_entries_refuse_before_any_launch():
+    lib = _lib.load()
+
+    def fwd(x=A, ldx=8, u=A, ldu=8, z=A, ldz=8, pg=A, pb=A, ng=A, nb=A, y=A, n=A, stats=A, rows=4, D=8, eps=1e-5, dtype=0, ptype=0):
+        return lib.mbvae_gated_norm_fwd(x, ldx, u, ldu, z, ldz, 0, 1.0, pg, pb, 0, ng, nb, y, n, stats, rows, D, 0, eps, dtype, ptype, 0)
+
+    def bwd(x=A, ldx=8, u=A, ldu=8, z=A, ldz=8, pg=A, pb=A, ng=A, stats=A, dn=A, lddn=8, du=A, dz=A, dpg=A, dng=A, rows=4, D=8, eps=1e-5, dtype=0,
+            ptype=0, ws=A, ws_bytes=1 << 20):
+        return lib.mbvae_gated_norm_bwd(x, ldx, u, ldu, z, ldz, 0, 1.0, pg, pb, 0, ng, stats, 0, 0, dn, lddn, A, du, dz, 0, dpg, 0, dng, 0, rows, D, 0,
+                                        eps, dtype, ptype, ws, ws_bytes, 0)
+
+    for call in (fwd, bwd):
+        assert call(x=0) == EINVAL and call(rows=-1) == EINVAL and call(D=0) == EINVAL and call(dtype=3) == EINVAL and call(ptype=-1) == EINVAL
+        assert call(ldx=-1) == EINVAL and call(ldu=-1) == EINVAL and call(ldz=-1) == EINVAL and call(eps=-1.0) == EINVAL and call(eps=math.nan) == EINVAL
+        assert call(D=8193) == EUNSUPPORTED and call(rows=1 << 31) == EUNSUPPORTED and call(pg=0, pb=A) == EINVAL and call(stats=A + 4) == EINVAL
+    assert fwd(y=0) == EINVAL and fwd(n=0) == EINVAL and fwd(ng=0) == EINVAL        # (a beta without its gamma)
+    assert fwd(rows=0, x=0) == 0
+    assert bwd(ng=0) == EINVAL and bwd(pg=0, pb=0) == EINVAL and bwd(u=0) == EINVAL and bwd(z=0) == EINVAL
+    assert bwd(stats=0) == EINVAL and bwd(lddn=-1) == EINVAL and bwd(ws=0) == EINVAL and bwd(ws=A + 8) == EINVAL
+    assert bwd(ws_bytes=lib.mbvae_gated_norm_bwd_workspace(4, 8, 0) - 1) == EINVAL
