@@ -7,6 +7,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmbvae_hip.so")
+HOST_SRC = os.path.join(CSRC, "host.cpp")                      # host code only: checks, allocation and autograd nodes of a few operators
+HOST_OUT = os.path.join(HERE, "mbvae_amd", "_host.so")
 SOURCES = ["gemm.hip", "edge_attn.hip", "edge_fused.hip", "rowops.hip", "loss.hip", "diffusion.hip", "eigen.hip", "cycles.hip",
            "gated_norm.hip", "embedding.hip", "gradclip.hip"]
 # No packed-fp32 instructions (v_pk_*_f32) in device code.  Measured on MI355X: the node-path LayerNorm backward
@@ -27,6 +29,19 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def host_command():
+    """The compiler call of the Python extension module (g++ against torch's headers; torch's libraries are in the process already
+    when it is imported, so their names are all it needs)."""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), "/opt/rocm/include",
+           sysconfig.get_paths()["include"]]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            "-DTORCH_EXTENSION_NAME=_host", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in inc),
+            HOST_SRC, "-o", HOST_OUT, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"]
+
+
 def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objdir = os.path.join(HERE, "build")
@@ -38,6 +53,9 @@ def build(force=False, verbose=True):
         o = os.path.join(objdir, src.replace(".hip", ".o"))
         if force or _stale(o, [s] + common):
             jobs.append([hipcc, *FLAGS, "-c", s, "-o", o])
+    kernels = bool(jobs)
+    if force or _stale(HOST_OUT, [HOST_SRC]):
+        jobs.insert(0, host_command())
 
     def run(cmd):
         if verbose:
@@ -52,7 +70,7 @@ def build(force=False, verbose=True):
     with ThreadPoolExecutor(max_workers=4) as ex:
         list(ex.map(run, jobs))
     objs = [os.path.join(objdir, s.replace(".hip", ".o")) for s in SOURCES]
-    if force or jobs or _stale(OUT, objs):
+    if force or kernels or _stale(OUT, objs):
         run([hipcc, "-shared", "-fPIC", "--offload-arch=gfx950", "-o", OUT, *objs])
     return OUT
 

@@ -104,6 +104,25 @@ def load():
     return lib
 
 
+_host = None
+
+
+def host():
+    """The extension module that checks arguments, allocates and holds the autograd nodes of the operators whose calls are short
+    (csrc/host.cpp), bound to the entry points of the library that load() has loaded; raises if it has not been built."""
+    global _host
+    if _host is None:
+        lib = load()
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise RuntimeError(f"mbvae_amd/_host.so cannot be loaded ({e}): build it first (python mb-vae-dti_amd/build.py). "
+                               "There is no fallback path.") from e
+        module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in SIGNATURES})
+        _host = module
+    return _host
+
+
 # When set to a dict, every kernel call is bracketed by HIP events on the current torch stream:
 # PROFILE[(name, tag)] = [(start_event, end_event), ...]   (used by bench.py for per-kernel timings)
 PROFILE = None

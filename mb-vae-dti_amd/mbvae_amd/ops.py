@@ -3,13 +3,10 @@
 Every function here requires CUDA(HIP) float32 tensors and calls libmbvae_hip.so through ctypes; nothing
 falls back to eager PyTorch arithmetic.
 """
-import array
-import contextlib
 import math
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -113,39 +110,6 @@ def _mask_u8(mask):
         return None
     m = mask if mask.is_contiguous() else mask.contiguous()
     return m.view(torch.uint8) if m.dtype == torch.bool else m.to(torch.uint8)
-
-
-# Tensor types of the operators that are not fp32 only (embedding, gated residual norm, gradient clipping), as the C ABI counts them
-_TYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _typed(t, name, dtype=None, device=None):
-    """Checks type and place of an operand; dtype / device: what it has to share with another one."""
-    if not t.is_cuda or t.dtype not in _TYPE_CODE:
-        raise RuntimeError(f"{name}: expected a float32, bfloat16 or float16 tensor on the GPU (got {t.dtype} on {t.device}); "
-                           "the HIP path has no CPU fallback")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name}: expected a tensor on {device}, got one on {t.device}")
-    return t
-
-
-def _rows(t, D):
-    """(t as [rows, D] with contiguous rows, elements between rows): a view where the layout allows one."""
-    r = t if t.dim() == 2 else t.reshape(-1, D)
-    if r.shape[0] == 0:
-        return r, D
-    if r.stride(1) != 1 and D > 1:
-        r = r.contiguous()
-    return r, r.stride(0) if r.shape[0] > 1 else D
-
-
-def _on_device(device):
-    """Makes the tensors' device current for a launch (streams and launches belong to the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
 
 
 # ------------------------------------------------------------------------------------------------ linear
@@ -397,62 +361,6 @@ def gate_update(x, u, z, drop_p=0.0, training=False):
 
 
 # ------------------------------------------------------------------------------------------------ gated residual norm
-def _gated_norm_fwd(x, u, z, keep, keep_scale, post_g, post_b, scale, pre_g, pre_b, rms, eps, want_stats):
-    D = x.shape[-1]
-    (x2, ldx), (u2, ldu), (z2, ldz) = ((None, 0) if t is None else _rows(t, D) for t in (x, u, z))
-    rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = torch.empty_like(y) if pre_g is not None else None
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if want_stats else None
-    param = next((t for t in (post_g, scale, pre_g) if t is not None), None)
-    with _on_device(x.device):
-        _lib.call("mbvae_gated_norm_fwd", x2.data_ptr(), ldx, _ptr(u2), ldu, _ptr(z2), ldz, _ptr(keep), keep_scale, _ptr(post_g), _ptr(post_b),
-                  _ptr(scale), _ptr(pre_g), _ptr(pre_b), y.data_ptr(), _ptr(n), _ptr(stats), rows, D, rms, eps, _TYPE_CODE[x.dtype],
-                  0 if param is None else _TYPE_CODE[param.dtype], _stream(), tag=(rows, D))
-    return y, n, stats, (x2, u2, z2)
-
-
-class _GatedResidualNorm(torch.autograd.Function):
-    """Nothing but the inputs and two statistics per norm and row are kept: the backward forms y again from what it reads anyway."""
-
-    @staticmethod
-    def forward(ctx, x, u, z, keep, keep_scale, post_g, post_b, scale, pre_g, pre_b, rms, eps):
-        y, n, stats, (x2, u2, z2) = _gated_norm_fwd(x, u, z, keep, keep_scale, post_g, post_b, scale, pre_g, pre_b, rms, eps, True)
-        ctx.save_for_backward(x2, u2, z2, keep, post_g, post_b, scale, pre_g, stats)
-        ctx.cfg = (keep_scale, pre_b is not None, rms, eps, x.shape)
-        ctx.set_materialize_grads(False)
-        return y, n
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dn):
-        x, u, z, keep, post_g, post_b, scale, pre_g, stats = ctx.saved_tensors
-        keep_scale, has_pre_b, rms, eps, shape = ctx.cfg
-        if dy is None and dn is None:
-            return (None,) * 12
-        rows, D = x.shape
-        need = ctx.needs_input_grad
-        lds = [D if t is None or rows <= 1 else t.stride(0) for t in (x, u, z)]
-        (dy2, lddy), (dn2, lddn) = ((None, 0) if t is None else _rows(_typed(t, "gradient", x.dtype, x.device), D) for t in (dy, dn))
-
-        def like(t, wanted, have=True):
-            return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted and have and t is not None else None
-
-        dx, du, dz = like(x, need[0]), like(u, need[1]), like(z, need[2])
-        dpost_g, dpost_b, dscale = like(post_g, need[5]), like(post_b, need[6]), like(scale, need[7])
-        dpre_g, dpre_b = like(pre_g, need[8]), like(pre_g, need[9], has_pre_b)
-        param = next((t for t in (post_g, scale, pre_g) if t is not None), None)
-        code = _TYPE_CODE[x.dtype]
-        ws = torch.empty(_lib.query("mbvae_gated_norm_bwd_workspace", rows, D, code), dtype=torch.uint8, device=x.device)
-        with _on_device(x.device):
-            _lib.call("mbvae_gated_norm_bwd", x.data_ptr(), lds[0], _ptr(u), lds[1], _ptr(z), lds[2], _ptr(keep), keep_scale, _ptr(post_g),
-                      _ptr(post_b), _ptr(scale), _ptr(pre_g), stats.data_ptr(), _ptr(dy2), lddy, _ptr(dn2), lddn, _ptr(dx), _ptr(du), _ptr(dz),
-                      _ptr(dscale), _ptr(dpost_g), _ptr(dpost_b), _ptr(dpre_g), _ptr(dpre_b), rows, D, rms, eps, code,
-                      0 if param is None else _TYPE_CODE[param.dtype], ws.data_ptr(), ws.numel(), _stream(), tag=(rows, D))
-        dx, du, dz = (t if t is None else t.view(shape) for t in (dx, du, dz))
-        return dx, du, dz, None, None, dpost_g, dpost_b, dscale, dpre_g, dpre_b, None, None
-
-
 def gated_residual_norm(x, u=None, z=None, keep=None, keep_scale=1.0, post=None, res_scale=None, pre=None, norm="layer", eps=1e-5):
     """What a residual block does around its products, in one kernel each way:
 
@@ -464,45 +372,13 @@ def gated_residual_norm(x, u=None, z=None, keep=None, keep_scale=1.0, post=None,
     res_scale: [D].  gamma, beta and res_scale share one type, float32 or any other of the three.  norm: "layer" or "rms".  Sums, statistics
     and intermediate values are float32, outputs are rounded once (n comes from the unrounded y).  1 <= D <= 8192.  The gate and
     norm of mb_vae_dti/training/models/blocks.py:92-129, :318-328 (gate_update and ln_residual are the separate forms)."""
-    _typed(x, "x")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
-        raise ValueError(f"gated_residual_norm: the last dimension must hold 1 to 8192 values, got shape {tuple(x.shape)}")
-    if norm not in ("layer", "rms"):
+    if norm != "layer" and norm != "rms":
         raise ValueError(f"gated_residual_norm: norm is 'layer' or 'rms', got {norm!r}")
-    if not eps >= 0:
-        raise ValueError("gated_residual_norm: eps must not be negative")
-    for name, t in (("u", u), ("z", z)):
-        if t is not None and _typed(t, name, x.dtype, x.device).shape != x.shape:
-            raise ValueError(f"gated_residual_norm: {name} must have x's shape {tuple(x.shape)}, got {tuple(t.shape)}")
-    if keep is not None:
-        if keep.shape != x.shape or keep.dtype not in (torch.uint8, torch.bool) or keep.device != x.device:
-            raise ValueError("gated_residual_norm: keep must be a uint8 or bool mask of x's shape on x's device")
-        keep = _mask_u8(keep)
-    (post_g, post_b), (pre_g, pre_b) = ((None, None) if p is None else p for p in (post, pre))
-    params = []
-    for name, t in (("post gamma", post_g), ("post beta", post_b), ("res_scale", res_scale), ("pre gamma", pre_g), ("pre beta", pre_b)):
-        if t is not None:
-            _typed(t, name, params[0].dtype if params else None, x.device)
-            if t.shape != (x.shape[-1],):
-                raise ValueError(f"gated_residual_norm: {name} must have shape ({x.shape[-1]},), got {tuple(t.shape)}")
-            t = t if t.is_contiguous() else t.contiguous()
-            params.append(t)
-        if name == "post gamma":
-            post_g = t
-        elif name == "post beta":
-            post_b = t
-        elif name == "res_scale":
-            res_scale = t
-        elif name == "pre gamma":
-            pre_g = t
-        else:
-            pre_b = t
+    post_g, post_b = post if post is not None else (None, None)
+    pre_g, pre_b = pre if pre is not None else (None, None)
     if (post is not None and post_g is None) or (pre is not None and pre_g is None):
         raise ValueError("gated_residual_norm: a norm needs its gamma")
-    args = (x, u, z, keep, float(keep_scale), post_g, post_b, res_scale, pre_g, pre_b, int(norm == "rms"), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, u, z, post_g, post_b, res_scale, pre_g, pre_b)):
-        return _GatedResidualNorm.apply(*args)
-    return _gated_norm_fwd(*args, False)[:2]
+    return _lib.host().gated_residual_norm(x, u, z, keep, keep_scale, post_g, post_b, res_scale, pre_g, pre_b, norm == "rms", eps)
 
 
 # ------------------------------------------------------------------------------------------------ edge-tensor fan-out
@@ -1250,108 +1126,23 @@ def dense_from_ids(atom_ids, bond_ids, cx, ce):
 
 
 # ------------------------------------------------------------------------------------------------ embedding
-_ID_CODE = {torch.int8: 1, torch.int16: 2, torch.uint8: 3, torch.int32: 4, torch.int64: 8}
-
-
-def _embedding_fwd(ids, weight, scale):
-    y = torch.empty((*ids.shape, weight.shape[1]), dtype=weight.dtype, device=weight.device)
-    with _on_device(weight.device):
-        _lib.call("mbvae_embedding_fwd", ids.data_ptr(), _ID_CODE[ids.dtype], weight.data_ptr(), y.data_ptr(), ids.numel(), *weight.shape, scale,
-                  _TYPE_CODE[weight.dtype], _stream(), tag=(ids.numel(), *weight.shape))
-    return y
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale):
-        ctx.save_for_backward(ids)
-        ctx.cfg = (weight.shape, scale)
-        return _embedding_fwd(ids, weight, scale)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        ids, = ctx.saved_tensors
-        (vocab, D), scale = ctx.cfg
-        dw = torch.empty((vocab, D), dtype=dy.dtype, device=dy.device)
-        if D == 0 or vocab == 0:
-            return None, dw, None
-        rows = ids.numel()
-        dy2, ldy = _rows(_typed(dy, "gradient"), D)
-        ws = torch.empty(_lib.query("mbvae_embedding_bwd_workspace", rows, vocab, D), dtype=torch.uint8, device=dy.device)
-        with _on_device(dy.device):
-            _lib.call("mbvae_embedding_bwd", ids.data_ptr(), _ID_CODE[ids.dtype], dy2.data_ptr(), ldy, dw.data_ptr(), rows, vocab, D, scale,
-                      _TYPE_CODE[dy.dtype], ws.data_ptr(), ws.numel(), _stream(), tag=(rows, vocab, D))
-        return None, dw, None
-
-
 def embedding(ids, weight, scale=1.0):
     """scale * weight[ids]: rows of a table by class id, ids of any shape (int8, int16, uint8, int32, int64), weight [V, D] (float32,
     bfloat16, float16) -> [*ids.shape, D].  Ids outside [0, V) - the -1 of padding in the class-id wire format - give a row of zeros and
     take no gradient.  The table's gradient sums the rows of equal ids in float32, in an order that the ids alone decide."""
-    _typed(weight, "weight")
-    if ids.dtype not in _ID_CODE or ids.device != weight.device:
-        raise RuntimeError(f"embedding: expected integer ids on {weight.device} (got {ids.dtype} on {ids.device}); the HIP path has no CPU fallback")
-    if weight.dim() != 2:
-        raise ValueError(f"embedding: weight must be [V, D], got shape {tuple(weight.shape)}")
-    if ids.numel() >= 1 << 31 or weight.shape[0] >= 1 << 31 or weight.shape[1] > 1 << 23:
-        raise ValueError("embedding: at most 2^31 - 1 ids, 2^31 - 1 table rows and 2^23 columns")
-    ids = ids if ids.is_contiguous() else ids.contiguous()
-    weight = weight if weight.is_contiguous() else weight.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return _Embedding.apply(ids, weight, float(scale))
-    return _embedding_fwd(ids, weight, float(scale))
+    return _lib.host().embedding(ids, weight, scale)
 
 
 # ------------------------------------------------------------------------------------------------ gradient norm and clipping
-def _check_gradients(grads, outs):
-    """Refuses what the kernels cannot take; returns the one device all tensors are on."""
-    devices = {t.get_device() for t in grads}
-    if len(devices) != 1 or -1 in devices:
-        raise RuntimeError("gradient norm: all gradients must be on one GPU; the HIP path has no CPU fallback")
-    for t in grads:
-        if t.dtype not in _TYPE_CODE:
-            raise RuntimeError(f"gradient norm: expected float32, bfloat16 or float16 gradients, got {t.dtype}")
-        if t.requires_grad:
-            raise ValueError("gradient norm: expected gradients (p.grad), got a tensor that requires gradients itself")
-    for t in grads if outs is grads else (*grads, *outs):
-        if not t.is_contiguous() and not torch._prims_common.is_non_overlapping_and_dense(t):
-            raise ValueError(f"gradient norm: a gradient must fill its memory densely, got strides {t.stride()} for shape {tuple(t.shape)}")
-    if outs is not grads:
-        for t, o in zip(grads, outs):
-            if o.dtype != t.dtype or o.shape != t.shape or o.get_device() != t.get_device() or (o.stride() != t.stride() and t.numel() > 1):
-                raise ValueError("clip_grad_norm_: an output must have its gradient's type, shape, strides and device")
-    return grads[0].device
-
-
-def _grad_clip(grads, outs, max_norm, norm_type):
-    if norm_type not in (1, 2, math.inf):
-        raise ValueError(f"gradient norm: norm_type is 1, 2 or infinity, got {norm_type}")
-    device = _check_gradients(grads, grads if outs is None else outs)
-    count = len(grads)
-    src = array.array("Q", [t.data_ptr() for t in grads])
-    dst = src if outs is grads else None if outs is None else array.array("Q", [t.data_ptr() for t in outs])
-    numel = array.array("q", [t.numel() for t in grads])
-    types = array.array("i", [_TYPE_CODE[t.dtype] for t in grads])
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    ws = torch.empty(_lib.query("mbvae_grad_clip_workspace", count), dtype=torch.uint8, device=device)
-    with _on_device(device):
-        _lib.call("mbvae_grad_clip", src.buffer_info()[0], 0 if dst is None else dst.buffer_info()[0], numel.buffer_info()[0],
-                  types.buffer_info()[0], count, float(norm_type), float(max_norm), norm.data_ptr(), ws.data_ptr(), ws.numel(), _stream(), tag=(count,))
-    return norm
-
-
-@torch.no_grad()
 def global_grad_norm(grads, norm_type=2.0):
     """(sum |g|^p)^(1/p) over all values of a list of gradients (None entries are skipped), p = 1, 2 or infinity: one float32 value on
     the GPU, without a host synchronisation.  Sums are float64."""
     grads = [g for g in grads if g is not None]
     if not grads:
         return torch.zeros((), device="cuda")
-    return _grad_clip(grads, None, 0.0, norm_type)
+    return _lib.host().grad_clip(grads, [], -1.0, norm_type)
 
 
-@torch.no_grad()
 def clip_grad_norm_(grads, max_norm, norm_type=2.0, out=None):
     """Scales a list of gradients (p.grad of a model's parameters; None entries are skipped) by min(1, max_norm / (norm + 1e-6)) and
     returns their norm before it as one float32 value on the GPU: what Lightning's gradient_clip_val does (mb_vae_dti/training/run.py:638-654).
@@ -1370,9 +1161,7 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, out=None):
     grads = [g for g in grads if g is not None]
     if not grads:
         return torch.zeros((), device="cuda")
-    norm = _grad_clip(grads, grads if outs is None else outs, max_norm, norm_type)
-    torch.autograd.graph.increment_version(grads if outs is None else outs)
-    return norm
+    return _lib.host().grad_clip(grads, outs or [], max_norm, norm_type)
 
 
 # ------------------------------------------------------------------------------------------------ diffusion samplers
