@@ -430,10 +430,10 @@ int mbvae_dense_from_ids(const int8_t* atoms, const int8_t* bonds, float* X, flo
  * give a row of zeros and take no gradient; nothing is read for them.
  * Backward: dweight[v] = scale * sum of dy[r] over the rows with ids[r] == v, zero where there are none; dy has rows ldy elements
  * apart.  Sums in fp32, in an order that the ids alone decide: bitwise reproducible.  workspace: at least
- * mbvae_embedding_bwd_workspace(rows, vocab, D) bytes, 16-byte aligned.  rows, vocab < 2^31, D <= 2^23. */
+ * mbvae_embedding_bwd_workspace(rows, vocab, D, dtype) bytes, 16-byte aligned.  rows, vocab < 2^31, D <= 2^23. */
 int mbvae_embedding_fwd(const void* ids, int id_type, const void* weight, void* y, int64_t rows, int64_t vocab, int64_t D,
                         float scale, int dtype, mbvae_stream_t stream);
-int64_t mbvae_embedding_bwd_workspace(int64_t rows, int64_t vocab, int64_t D);
+int64_t mbvae_embedding_bwd_workspace(int64_t rows, int64_t vocab, int64_t D, int dtype);
 int mbvae_embedding_bwd(const void* ids, int id_type, const void* dy, int64_t ldy, void* dweight, int64_t rows, int64_t vocab,
                         int64_t D, float scale, int dtype, void* workspace, int64_t ws_bytes, mbvae_stream_t stream);
 

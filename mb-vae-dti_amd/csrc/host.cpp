@@ -29,7 +29,7 @@ struct Library {
                         const void*, const float*, const void*, int64_t, const void*, int64_t, void*, void*, void*, void*, void*, void*, void*, void*,
                         int64_t, int64_t, int, float, int, int, void*, int64_t, mbvae_stream_t);
   int (*embedding_fwd)(const void*, int, const void*, void*, int64_t, int64_t, int64_t, float, int, mbvae_stream_t);
-  int64_t (*embedding_bwd_workspace)(int64_t, int64_t, int64_t);
+  int64_t (*embedding_bwd_workspace)(int64_t, int64_t, int64_t, int);
   int (*embedding_bwd)(const void*, int, const void*, int64_t, void*, int64_t, int64_t, int64_t, float, int, void*, int64_t, mbvae_stream_t);
   int64_t (*grad_clip_workspace)(int64_t);
   int (*grad_clip)(const void* const*, void* const*, const int64_t*, const int32_t*, int64_t, double, double, float*, void*, int64_t, mbvae_stream_t);
@@ -143,7 +143,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     Tensor dw = at::empty({vocab, D}, dy.options().requires_grad(false));
     if (vocab > 0 && D > 0) {
       const Rows d(dy, D);
-      const Tensor ws = bytes_on(dy, lib.embedding_bwd_workspace(rows, vocab, D));
+      const Tensor ws = bytes_on(dy, lib.embedding_bwd_workspace(rows, vocab, D, type_code(dy.scalar_type())));
       const c10::DeviceGuard guard(dy.device());
       succeeded(lib.embedding_bwd(ids.const_data_ptr(), id_code(ids.scalar_type()), d.t.const_data_ptr(), d.ld, dw.mutable_data_ptr(), rows, vocab, D,
                                   (float)ctx->saved_data["scale"].toDouble(), type_code(dy.scalar_type()), ws.mutable_data_ptr(), ws.numel(),

@@ -40,6 +40,20 @@ __device__ __forceinline__ void mbvae_load_vec(const T* p, int64_t left, float* 
   }
 }
 
+// The same as one vector of the type itself.
+template <typename T>
+__device__ __forceinline__ typename MbvaeVec<T>::Aligned mbvae_load_raw(const T* p, int64_t left) {
+  constexpr int N = MbvaeVec<T>::N;
+  typename MbvaeVec<T>::Aligned t;
+  if (left >= N) {
+    t = *reinterpret_cast<const typename MbvaeVec<T>::Any*>(p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) t[e] = e < left ? p[e] : (T)0.f;
+  }
+  return t;
+}
+
 // The first min(N, left) elements at p = v, each rounded once to nearest even.
 template <typename T>
 __device__ __forceinline__ void mbvae_store_vec(T* p, int64_t left, const float* v) {

@@ -70,7 +70,7 @@ SIGNATURES = {
     "mbvae_gated_norm_bwd": [_P, _L, _P, _L, _P, _L, _P, _F] + [_P] * 5 + [_P, _L, _P, _L] + [_P] * 8
                             + [_L, _L, _I, _F, _I, _I, _P, _L, _P],
     "mbvae_embedding_fwd": [_P, _I, _P, _P, _L, _L, _L, _F, _I, _P],
-    "mbvae_embedding_bwd_workspace": [_L, _L, _L],
+    "mbvae_embedding_bwd_workspace": [_L, _L, _L, _I],
     "mbvae_embedding_bwd": [_P, _I, _P, _L, _P, _L, _L, _L, _F, _I, _P, _L, _P],
     "mbvae_grad_clip_workspace": [_L],
     "mbvae_grad_clip": [_P, _P, _P, _P, _L, c_double, c_double, _P, _P, _L, _P],

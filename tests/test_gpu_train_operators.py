@@ -53,7 +53,9 @@ EMBEDDING = [
     (8191, 700, 12, F32, torch.int64, "hot"), (8192, 70000, 9, F32, torch.int32, "uniform"), (8193, 300, 24, BF16, torch.int64, "uniform"),
     (20000, 5, 64, F32, torch.int8, "hot"), (20000, 4170, 48, F16, torch.int32, "sorted"), (40000, 3, 16, F32, torch.int8, "one"),
     (70001, 66000, 20, F32, torch.int64, "hot"), (30000, 9, 1037, BF16, torch.int8, "uniform"), (16385, 11, 8, F32, torch.int8, "none"),
-    (17, 20, 2050, F32, torch.int64, "uniform"), (5000, 1, 40, F32, torch.int64, "uniform"),
+    (17, 20, 2050, F32, torch.int64, "uniform"), (700, 32, 260, F32, torch.int8, "hot"), (700, 33, 260, F32, torch.int8, "hot"), (3000, 16, 520, BF16, torch.int16, "uniform"),
+    (3000, 17, 520, BF16, torch.uint8, "hot"), (32768, 4000, 16, F32, torch.int64, "hot"), (32769, 4000, 16, F32, torch.int64, "hot"), (32768, 33, 8, F16, torch.int8, "one"),
+    (900, 65535, 8, F32, torch.int32, "uniform"), (900, 65536, 8, F32, torch.int64, "uniform"), (2, 65000, 4, BF16, torch.int64, "uniform"), (5000, 1, 40, F32, torch.int64, "uniform"),
 ]
 
 
@@ -77,6 +79,27 @@ def test_embedding_forward_and_gradient(ops, rows, V, D, dtype, id_dtype, kind):
     y = ops.embedding(ids.cuda(), weight, scale)
     again, = torch.autograd.grad(y, weight, dy.cuda())
     assert torch.equal(again, dw), "the same call gives other bits"
+
+
+@pytest.mark.parametrize("lengths", [[16], [16, 16], [32, 16], [15, 17, 16], [33, 1, 14], [1, 15, 16, 48], [47, 17], [31, 1, 1, 31], [5, 16, 11, 16, 16], [64, 1],
+                                     [8, 40, 16], [17, 47, 1, 16], [16, 17, 15, 1, 33, 14, 80, 3], [160, 160, 7], [1] * 50, [2, 30] * 8, [129, 255, 1, 127]])
+@pytest.mark.parametrize("many", [False, True])
+def test_embedding_gradient_runs_meet_chunks(ops, lengths, many):
+    """Runs of equal ids that begin and end on, before and behind multiples of 16 tokens, at the end of the tokens and before padding; with
+    `many` behind 33 000 tokens of smaller ids, which take the radix sort and another chunk length."""
+    g = _gen(len(lengths) + sum(lengths))
+    V, D = 1000, 24
+    ids = torch.cat([torch.full((n,), 40 + 3 * k) for k, n in enumerate(lengths)])
+    if many:
+        ids = torch.cat((torch.arange(33 * 1024) % 33, ids))
+    for pad in (0, 1, 16, 21):
+        every = torch.cat((ids, torch.full((pad,), -1)))
+        every = every[torch.randperm(every.numel(), generator=g)]
+        dy = _randn(g, every.numel(), D)
+        weight = _randn(g, V, D).cuda().requires_grad_(True)
+        dw, = torch.autograd.grad(ops.embedding(every.cuda(), weight, 0.5), weight, dy.cuda())
+        want, bound = embedding_gradient(every, dy, V, 0.5)
+        check(dw, want, bound, f"dweight, {pad} rows of padding")
 
 
 def test_embedding_shapes_strides_and_ids_outside(ops):
@@ -634,7 +657,7 @@ def test_outputs_end_where_they_end(ops):
             ids = torch.randint(0, rows, (rows,), generator=g).cuda()
             _lib.call("mbvae_embedding_fwd", ids.data_ptr(), 8, x.data_ptr(), mid.data_ptr(), rows, rows, D, 1.0, code, st)
             assert torch.equal(mid.view(rows, D), x[ids]) and bool((buf[:guard] == 3).all()) and bool((buf[guard + size:] == 3).all())
-            ws = torch.empty(_lib.query("mbvae_embedding_bwd_workspace", rows, rows, D), dtype=torch.uint8, device="cuda")
+            ws = torch.empty(_lib.query("mbvae_embedding_bwd_workspace", rows, rows, D, code), dtype=torch.uint8, device="cuda")
             _lib.call("mbvae_embedding_bwd", ids.data_ptr(), 8, x.data_ptr(), D, mid.data_ptr(), rows, rows, D, 1.0, code, ws.data_ptr(), ws.numel(), st)
             check(mid.view(rows, D), *embedding_gradient(ids, x, rows, 1.0), "dweight")
             assert bool((buf[:guard] == 3).all()) and bool((buf[guard + size:] == 3).all())

@@ -84,7 +84,7 @@ def test_embedding_entries_refuse_before_any_launch():
     assert fwd(rows=0, ids=0, y=0) == 0 and fwd(D=0) == 0
     assert bwd(dy=0) == EINVAL and bwd(dw=0) == EINVAL and bwd(ldy=-1) == EINVAL
     assert bwd(ws=0) == EINVAL and bwd(ws=A + 8) == EINVAL
-    assert bwd(ws_bytes=lib.mbvae_embedding_bwd_workspace(4, 5, 8) - 1) == EINVAL
+    assert bwd(ws_bytes=lib.mbvae_embedding_bwd_workspace(4, 5, 8, 0) - 1) == EINVAL
     assert bwd(vocab=0) == 0 and bwd(D=0) == 0
 
 
