@@ -10,7 +10,7 @@ OUT = os.path.join(HERE, "libmbvae_hip.so")
 HOST_SRC = os.path.join(CSRC, "host.cpp")                      # host code only: checks, allocation and autograd nodes of a few operators
 HOST_OUT = os.path.join(HERE, "mbvae_amd", "_host.so")
 SOURCES = ["gemm.hip", "edge_attn.hip", "edge_fused.hip", "rowops.hip", "loss.hip", "diffusion.hip", "eigen.hip", "cycles.hip",
-           "gated_norm.hip", "embedding.hip", "gradclip.hip"]
+           "gated_norm_f32.hip", "gated_norm_bf16.hip", "gated_norm_f16.hip", "gated_norm.hip", "embedding.hip", "gradclip.hip"]
 # No packed-fp32 instructions (v_pk_*_f32) in device code.  Measured on MI355X: the node-path LayerNorm backward
 # (ln_res_bwd_kernel<64, 1>), whose compiled form reads its per-row statistics through op_sel'ed packed operands, returned
 # rare wrong rows (the low half of one packed subtract behaving as "minus 0" in lanes 48-63) whenever tall-skinny product
@@ -46,7 +46,7 @@ def build(force=False, verbose=True):
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    common = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "typed.h")]
+    common = [os.path.join(CSRC, h) for h in ("common.h", "typed.h", "gated_norm.h", "gated_norm_kernels.h")]
     jobs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)

@@ -92,7 +92,8 @@ __global__ __launch_bounds__(256) void embedding_few_kernel(const void* __restri
   constexpr int N = MbvaeVec<T>::N, U = 4;
   extern __shared__ float4 cell[];
   const int teams = 256 / lanes, team = threadIdx.x / lanes, lane = threadIdx.x % lanes;
-  const int64_t col = ((int64_t)blockIdx.y * lanes + lane) * N, left = D - col;
+  const int64_t col = ((int64_t)blockIdx.y * lanes + lane) * N;
+  const int left = (int)(D - col);
   for (uint32_t i = threadIdx.x; i < V * (N / 4) * 256; i += 256) cell[i] = make_float4(0.f, 0.f, 0.f, 0.f);      // (a thread clears its own)
   const int64_t stride = (int64_t)gridDim.x * teams;
   if (left > 0) {
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_order_kernel(const voi
   const float zero[MbvaeVec<T>::N] = {};
   for (uint32_t k = lo + wave; k < min(hi, V); k += SORT_WAVES)
     if (total[k - lo] == 0)
-      for (int64_t c = (int64_t)lane * MbvaeVec<T>::N; c < D; c += 64 * MbvaeVec<T>::N) mbvae_store_vec<T>(dW + (int64_t)k * D + c, D - c, zero);
+      for (int64_t c = (int64_t)lane * MbvaeVec<T>::N; c < D; c += 64 * MbvaeVec<T>::N) mbvae_store_vec<T>(dW + (int64_t)k * D + c, (int)(D - c), zero);
 }
 
 // ------------------------------------------------------------------------------------------------ many tokens: radix sort
@@ -404,7 +405,8 @@ __global__ __launch_bounds__(256) void embedding_runs_kernel(const uint32_t* __r
   const int64_t c = (int64_t)blockIdx.x * teams + team;
   const int64_t col = ((int64_t)blockIdx.y * lanes + lane) * N;
   if (c >= chunks || col >= D) return;
-  const int64_t begin = c * chunk, end = min(rows, begin + chunk), far = min(rows, end + chunk), left = D - col;
+  const int64_t begin = c * chunk, end = min(rows, begin + chunk), far = min(rows, end + chunk);
+  const int left = (int)(D - col);
   // the first tokens, and the keys at both ends of this chunk and its neighbours: all on their way before any is looked at
   uint32_t k[AHEAD], p[AHEAD];
 #pragma unroll
@@ -487,7 +489,8 @@ __global__ __launch_bounds__(64 * JOIN_GROUPS) void embedding_join_kernel(const 
   __shared__ float4 red[JOIN_GROUPS][64];
   const int lane = threadIdx.x & 63, group = threadIdx.x >> 6;
   for (int64_t col0 = JOIN_COLUMNS * (int64_t)blockIdx.y; col0 < D; col0 += JOIN_COLUMNS * (int64_t)gridDim.y) {
-    const int64_t col = col0 + 4 * lane, left = D - col;
+    const int64_t col = col0 + 4 * lane;
+    const int left = (int)(D - col);
     float s[U][4] = {};
     if (left > 0) {
       if (group == 0) mbvae_load_vec<float>(part + (c * 2 + 1) * D + col, left, s[0]);

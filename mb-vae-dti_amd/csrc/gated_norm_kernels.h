@@ -1,0 +1,414 @@
+// Kernels of the gated residual update (see gated_norm.hip for the mathematics) for one activation type.
+#pragma once
+#include "gated_norm.h"
+#include <type_traits>
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------ sums over a row
+// TPR lanes of a wave own a row (16, 32, 64), or, with TPR == 0, a whole block does: its waves meet in LDS, in buffers that alternate so
+// that one barrier a sum is enough.
+template <int TPR>
+struct Team {
+  float2* red;            // [2][16], used by whole blocks
+  int turn;
+  __device__ __forceinline__ float2 sum(float a, float b) {
+    if constexpr (TPR > 0) {
+      return make_float2(mbvae_team_sum<TPR>(a), mbvae_team_sum<TPR>(b));
+    } else {
+      a = mbvae_team_sum<64>(a);
+      b = mbvae_team_sum<64>(b);
+      float2* r = red + turn * 16;
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = make_float2(a, b);
+      __syncthreads();
+      float2 s = r[0];
+      for (unsigned w = 1; w < blockDim.x / 64; ++w) { s.x += r[w].x; s.y += r[w].y; }
+      return s;
+    }
+  }
+  __device__ __forceinline__ float sum(float a) {
+    if constexpr (TPR > 0) return mbvae_team_sum<TPR>(a);
+    else return sum(a, 0.f).x;
+  }
+};
+
+// 1 / a to within a rounding: the hardware's reciprocal and one Newton step.
+__device__ __forceinline__ float reciprocal(float a) {
+  const float r = __builtin_amdgcn_rcpf(a);
+  return fmaf(fmaf(-a, r, 1.f), r, r);
+}
+// sigmoid(z) and its derivative, accurate at both ends: with t = exp(-|z|) they are 1 / (1 + t) or t / (1 + t), and t / (1 + t)^2.
+// t = 2^-(h + l) where h + l is |z| log2(e) to 48 bits: the hardware's 2^h, corrected by l to first order.
+__device__ __forceinline__ void sigmoid(float z, float& s, float& ds) {
+  const float a = fabsf(z), h = a * 1.44269502f, l = fmaf(a, 1.44269502f, -h) + a * 1.92596299e-8f;
+  const float t0 = __builtin_amdgcn_exp2f(-h), t = a < 128.f ? fmaf(t0 * -0.693147181f, l, t0) : t0;      // (from 128 on l may not be finite)
+  const float r = reciprocal(1.f + t);
+  s = z < 0.f ? t * r : r;
+  ds = t * r * r;
+}
+
+// ------------------------------------------------------------------------------------------------ one thread's elements of a row
+// EPL of them in 16-byte pieces; piece v of thread l begins at column (v * width + l) * N.  ALIGNED: the row is a whole number of
+// pieces, so that a piece is inside it or not; otherwise the last piece is taken element by element.
+template <typename T, int TPR, int EPL, bool ALIGNED>
+struct Row {
+  static constexpr int N = MbvaeVec<T>::N, NV = EPL / N;
+  static_assert(NV * N == EPL, "whole pieces");
+  typedef typename MbvaeVec<T>::Aligned Piece;
+  int lane, width, D;
+  __device__ __forceinline__ Row(int columns) : lane(TPR ? threadIdx.x % (TPR ? TPR : 1) : threadIdx.x), width(TPR ? TPR : blockDim.x), D(columns) {}
+  __device__ __forceinline__ int col(int v) const { return (v * width + lane) * N; }
+  __device__ __forceinline__ bool inside(int e) const { return ALIGNED ? col(e / N) < D : col(e / N) + e % N < D; }
+
+  // `on`: whether the row is there at all (a team behind the last row has zeros for all it loads)
+  __device__ __forceinline__ void load(const void* p, int64_t at, bool on, Piece* out) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = col(v), left = on ? D - c : 0;
+      const T* q = reinterpret_cast<const T*>(p) + at + c;
+      if (ALIGNED) {
+        Piece t = {};
+        if (left > 0) t = *reinterpret_cast<const typename MbvaeVec<T>::Any*>(q);
+        out[v] = t;
+      } else {
+        out[v] = mbvae_load_raw<T>(q, left);
+      }
+    }
+  }
+  static __device__ __forceinline__ void widen(const Piece* in, float* out) {
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) out[e] = (float)in[e / N][e % N];
+  }
+  __device__ __forceinline__ void store(void* p, int64_t at, bool on, const float* val) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = col(v), left = on ? D - c : 0;
+      T* q = reinterpret_cast<T*>(p) + at + c;
+      if (ALIGNED) {
+        if (left > 0) mbvae_store_vec<T>(q, N, val + v * N);
+      } else {
+        mbvae_store_vec<T>(q, left, val + v * N);
+      }
+    }
+  }
+  // a vector over the columns in the parameters' type; `none` where p is null
+  template <typename P>
+  __device__ __forceinline__ void param_of(const P* p, float* out) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int q = 0; q < N; q += (N < MbvaeVec<P>::N ? N : MbvaeVec<P>::N)) {
+        constexpr int M = MbvaeVec<P>::N;
+        const int c = col(v) + q;
+        if constexpr (M <= N) {
+          mbvae_load_vec<P>(p + c, D - c, out + v * N + q);
+        } else {
+          float t[M];
+          mbvae_load_vec<P>(p + c, D - c < N ? D - c : N, t);            // (N of a longer piece)
+#pragma unroll
+          for (int e = 0; e < N; ++e) out[v * N + q + e] = t[e];
+        }
+      }
+  }
+  __device__ __forceinline__ void param(const void* p, int type, float none, float* out) const {
+    if (!p) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) out[e] = none;
+    } else if (type == MBVAE_F32) param_of(reinterpret_cast<const float*>(p), out);
+    else if (type == MBVAE_BF16) param_of(reinterpret_cast<const mbvae_bf16*>(p), out);
+    else param_of(reinterpret_cast<const mbvae_f16*>(p), out);
+  }
+  typedef uint8_t Bytes __attribute__((ext_vector_type(MbvaeVec<T>::N)));
+  typedef Bytes AnyBytes __attribute__((aligned(1)));
+  __device__ __forceinline__ void keep(const uint8_t* p, int64_t at, bool on, Bytes* out) const {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = col(v), left = on ? D - c : 0;
+      Bytes b = {};
+      if (left >= N) b = *reinterpret_cast<const AnyBytes*>(p + at + c);
+      else if (!ALIGNED)
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (e < left) b[e] = p[at + c + e];
+      out[v] = b;
+    }
+  }
+};
+
+// Mean and reciprocal deviation of a row (two-pass: the deviations are summed from the mean).
+template <int EPL, typename R, typename TeamT>
+__device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float* t, float inv_D, bool rms, float eps, float& mean, float& r) {
+  mean = 0.f;
+  if (!rms) {
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) s += t[e];
+    mean = team.sum(s) * inv_D;
+  }
+  float q = 0.f;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    const float d = row.inside(e) ? t[e] - mean : 0.f;
+    q = fmaf(d, d, q);
+  }
+  r = 1.f / sqrtf(fmaf(team.sum(q), inv_D, eps));
+}
+
+// Both kernels walk over the rows with a fixed grid and ask for the next row's operands before the current row's results are stored: a
+// load behind a store would wait for it (one counter, in order).
+template <typename T, int TPR, int EPL, int THREADS, bool ALIGNED>
+__global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a) {
+  typedef Row<T, TPR, EPL, ALIGNED> R;
+  constexpr int TEAMS = TPR ? THREADS / (TPR ? TPR : 1) : 1, NV = R::NV;
+  __shared__ float2 red[32];
+  Team<TPR> team{red, 0};
+  const R row(a.D);
+  const float inv_D = 1.f / a.D;
+  float pg[EPL], pb[EPL], ng[EPL], nb[EPL], sc[EPL];
+  row.param(a.post_g, a.ptype, 0.f, pg);
+  row.param(a.post_b, a.ptype, 0.f, pb);
+  row.param(a.pre_g, a.ptype, 0.f, ng);
+  row.param(a.pre_b, a.ptype, 0.f, nb);
+  row.param(a.scale, a.ptype, 1.f, sc);
+  const int64_t stride = (int64_t)gridDim.x * TEAMS;
+  int64_t base = (int64_t)blockIdx.x * TEAMS, r = base + (TPR ? threadIdx.x / (TPR ? TPR : 1) : 0);
+  typename R::Piece xn[NV], un[NV], zn[NV];
+  typename R::Bytes kn[NV];
+  const auto ask = [&]() {
+    const bool on = r < a.rows;
+    row.load(a.x, r * a.ldx, on, xn);
+    if (a.u) row.load(a.u, r * a.ldu, on, un);
+    if (a.z) row.load(a.z, r * a.ldz, on, zn);
+    if (a.keep) row.keep(a.keep, r * a.D, on, kn);
+  };
+  ask();
+  for (; base < a.rows; base += stride) {
+    const bool on = r < a.rows;
+    const int64_t at = r * a.D, mine = r;
+    float y[EPL], v[EPL], w[EPL];
+    R::widen(xn, y);
+    if (a.u) R::widen(un, v);
+    else
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) v[e] = y[e];
+    if (a.z) {
+      R::widen(zn, w);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) { float ds; sigmoid(w[e], w[e], ds); }
+    } else
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) w[e] = 1.f;
+    typename R::Bytes kept[NV];
+    if (a.keep)
+#pragma unroll
+      for (int q = 0; q < NV; ++q) kept[q] = kn[q];
+    r += stride;
+    if (base + stride < a.rows) ask();
+    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (a.post_g) {
+      row_stats<EPL>(row, team, v, inv_D, a.rms, a.eps, st.x, st.y);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) v[e] = fmaf((v[e] - st.x) * st.y, pg[e], pb[e]);
+    }
+    if (a.keep) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e)                                 // a dropped value adds nothing, whatever it is
+        y[e] = kept[e / R::N][e % R::N] ? fmaf(v[e] * (w[e] * a.keep_scale), sc[e], y[e]) : y[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) y[e] = fmaf(v[e] * w[e], sc[e], y[e]);
+    }
+    row.store(a.y, at, on, y);
+    if (a.pre_g) {
+      row_stats<EPL>(row, team, y, inv_D, a.rms, a.eps, st.z, st.w);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) y[e] = fmaf((y[e] - st.z) * st.w, ng[e], nb[e]);
+      row.store(a.n, at, on, y);
+    }
+    if (a.stats && on && row.lane == 0) a.stats[mine] = st;
+  }
+}
+
+template <typename T, int TPR, int EPL, int THREADS, bool ALIGNED>
+__global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a) {
+  typedef Row<T, TPR, EPL, ALIGNED> R;
+  constexpr int TEAMS = TPR ? THREADS / (TPR ? TPR : 1) : 1, NV = R::NV;
+  __shared__ float2 red[32];
+  __shared__ float join[TEAMS > 1 ? THREADS * EPL : 1];
+  Team<TPR> team{red, 0};
+  const R row(a.D);
+  const float inv_D = 1.f / a.D, mean_weight = a.rms ? 0.f : inv_D;
+  const bool post = a.post_g != nullptr, pre = a.pre_g != nullptr && a.dn != nullptr;
+  float pg[EPL], pb[EPL], ng[EPL], sc[EPL];
+  row.param(a.post_g, a.ptype, 0.f, pg);
+  row.param(a.post_b, a.ptype, 0.f, pb);
+  row.param(a.pre_g, a.ptype, 0.f, ng);
+  row.param(a.scale, a.ptype, 1.f, sc);
+  float sums[GATED_SUMS][EPL];
+#pragma unroll
+  for (int s = 0; s < GATED_SUMS; ++s)
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) sums[s][e] = 0.f;
+  const int64_t stride = (int64_t)gridDim.x * TEAMS;
+  int64_t base = (int64_t)blockIdx.x * TEAMS, r = base + (TPR ? threadIdx.x / (TPR ? TPR : 1) : 0);
+  typename R::Piece xn[NV], un[NV], zn[NV], tn[NV], dn[NV];
+  typename R::Bytes kn[NV];
+  float4 sn = make_float4(0.f, 0.f, 0.f, 0.f);
+  const auto ask = [&]() {
+    const bool on = r < a.rows;
+    sn = on ? a.stats[r] : make_float4(0.f, 0.f, 0.f, 0.f);
+    row.load(a.x, r * a.ldx, on, xn);
+    if (a.u) row.load(a.u, r * a.ldu, on, un);
+    if (a.z) row.load(a.z, r * a.ldz, on, zn);
+    if (a.dy) row.load(a.dy, r * a.lddy, on, tn);
+    if (pre) row.load(a.dn, r * a.lddn, on, dn);
+    if (a.keep) row.keep(a.keep, r * a.D, on, kn);
+  };
+  if (base < a.rows) ask();
+  for (; base < a.rows; base += stride) {
+    const bool on = r < a.rows;
+    const int64_t at = r * a.D;
+    const float4 st = sn;
+    float x[EPL], v[EPL], w[EPL], dw[EPL], t[EPL], d[EPL];
+    R::widen(xn, x);
+    if (a.u) R::widen(un, v);
+    else
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) v[e] = x[e];
+    if (a.z) R::widen(zn, w);
+    if (a.dy) R::widen(tn, t);
+    else
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) t[e] = 0.f;
+    if (pre) R::widen(dn, d);
+    bool kept[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) kept[e] = !a.keep || kn[e / R::N][e % R::N] != 0;
+    r += stride;
+    if (base + stride < a.rows) ask();
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      if (a.z) sigmoid(w[e], w[e], dw[e]);
+      else { w[e] = 1.f; dw[e] = 0.f; }
+      if (a.keep) {
+        w[e] = kept[e] ? w[e] * a.keep_scale : 0.f;
+        dw[e] = kept[e] ? dw[e] * a.keep_scale : 0.f;
+      }
+      if (post) v[e] = row.inside(e) ? (v[e] - st.x) * st.y : 0.f;          // normalised
+    }
+    if (pre) {
+      float g[EPL], hat[EPL], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float vv = post ? fmaf(v[e], pg[e], pb[e]) : v[e];
+        const float y = kept[e] ? fmaf(vv * w[e], sc[e], x[e]) : x[e];
+        hat[e] = row.inside(e) ? (y - st.z) * st.w : 0.f;
+        g[e] = d[e] * ng[e];
+        s1 += g[e];
+        s2 = fmaf(g[e], hat[e], s2);
+        sums[GATED_SUM_PRE_G][e] = fmaf(d[e], hat[e], sums[GATED_SUM_PRE_G][e]);
+        sums[GATED_SUM_PRE_B][e] += d[e];
+      }
+      const float2 m = team.sum(s1, s2);
+      const float m1 = m.x * mean_weight, m2 = m.y * inv_D;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) t[e] = fmaf(st.w, g[e] - fmaf(hat[e], m2, m1), t[e]);
+    }
+    // t is the whole gradient of y
+    float dv[EPL];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      const float vv = post ? fmaf(v[e], pg[e], pb[e]) : v[e];
+      dv[e] = kept[e] ? t[e] * sc[e] * w[e] : 0.f;
+      dw[e] = kept[e] ? t[e] * sc[e] * vv * dw[e] : 0.f;
+      sums[GATED_SUM_SCALE][e] += kept[e] ? t[e] * w[e] * vv : 0.f;
+      if (post) {
+        sums[GATED_SUM_POST_G][e] = fmaf(dv[e], v[e], sums[GATED_SUM_POST_G][e]);
+        sums[GATED_SUM_POST_B][e] += dv[e];
+      }
+    }
+    if (a.dz) row.store(a.dz, at, on, dw);
+    if (post) {
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        dv[e] = row.inside(e) ? dv[e] * pg[e] : 0.f;
+        s1 += dv[e];
+        s2 = fmaf(dv[e], v[e], s2);
+      }
+      const float2 m = team.sum(s1, s2);
+      const float m1 = m.x * mean_weight, m2 = m.y * inv_D;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) dv[e] = st.y * (dv[e] - fmaf(v[e], m2, m1));
+    }
+    if (a.u) {
+      if (a.du) row.store(a.du, at, on, dv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) t[e] += dv[e];
+    }
+    if (a.dx) row.store(a.dx, at, on, t);
+  }
+  // column sums of the block: its teams in order
+  float* part = a.part + (int64_t)blockIdx.x * GATED_SUMS * a.D;
+#pragma unroll
+  for (int s = 0; s < GATED_SUMS; ++s) {
+    if (s == GATED_SUM_SCALE ? !a.scale : s <= GATED_SUM_POST_B ? !post : !pre) {
+      if (s < GATED_SUM_PRE_G || a.pre_g == nullptr) continue;        // (a norm in front without a gradient behind it: its sums are zero)
+    }
+    if constexpr (TEAMS > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) join[e * THREADS + threadIdx.x] = sums[s][e];
+      __syncthreads();
+      if (threadIdx.x < TPR) {
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+          float total = 0.f;
+#pragma unroll
+          for (int k = 0; k < TEAMS; ++k) total += join[e * THREADS + k * TPR + threadIdx.x];
+          sums[s][e] = total;
+        }
+      }
+    }
+    if (TEAMS == 1 || threadIdx.x < TPR)
+#pragma unroll
+      for (int e = 0; e < EPL; ++e)
+        if (row.inside(e)) part[(int64_t)s * a.D + row.col(e / R::N) + e % R::N] = sums[s][e];
+  }
+}
+
+// f(threads a row within a wave or 0, elements, the block's most threads, aligned), all constants.
+template <typename T, typename F>
+void for_shape(int dtype, int D, F f) {
+  constexpr int N = MbvaeVec<T>::N;
+  const GatedNormShape s = gated_norm_shape(dtype, D);
+  const auto with = [&](auto lanes, auto elements, auto threads) {
+    if (D % N == 0) f(lanes, elements, threads, std::true_type());
+    else f(lanes, elements, threads, std::false_type());
+  };
+#define GN_CASE(lanes, elements, threads) \
+  with(std::integral_constant<int, lanes>(), std::integral_constant<int, elements>(), std::integral_constant<int, threads>())
+  if (s.threads_a_row == 16) GN_CASE(16, N, 256);
+  else if (s.threads_a_row == 32) GN_CASE(32, N, 256);
+  else if (s.threads_a_row == 64 && s.elements == N) GN_CASE(64, N, 256);
+  else if (s.threads_a_row == 64) GN_CASE(64, 8, 256);
+  else if (s.block <= 256) GN_CASE(0, 8, 256);
+  else if (s.block <= 512) GN_CASE(0, 8, 512);
+  else GN_CASE(0, 8, 1024);
+#undef GN_CASE
+}
+
+template <typename T>
+void gated_norm_launch(int dtype, bool forward, const GatedNormArgs& a, unsigned blocks, hipStream_t stream) {
+  const unsigned threads = (unsigned)gated_norm_shape(dtype, a.D).block;
+  for_shape<T>(dtype, a.D, [&](auto lanes, auto elements, auto most, auto aligned) {
+    constexpr int TPR = decltype(lanes)::value, EPL = decltype(elements)::value, MOST = decltype(most)::value;
+    constexpr bool ALIGNED = decltype(aligned)::value;
+    if (forward) hipLaunchKernelGGL((gated_norm_fwd_kernel<T, TPR, EPL, MOST, ALIGNED>), dim3(blocks), dim3(threads), 0, stream, a);
+    else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, TPR, EPL, MOST, ALIGNED>), dim3(blocks), dim3(threads), 0, stream, a);
+  });
+}
+
+}  // namespace

@@ -28,7 +28,7 @@ struct MbvaeVec {
 
 // v[0..N) = the N elements at p as fp32; those from `left` on are not read and become 0.
 template <typename T>
-__device__ __forceinline__ void mbvae_load_vec(const T* p, int64_t left, float* v) {
+__device__ __forceinline__ void mbvae_load_vec(const T* p, int left, float* v) {
   constexpr int N = MbvaeVec<T>::N;
   if (left >= N) {
     const typename MbvaeVec<T>::Aligned t = *reinterpret_cast<const typename MbvaeVec<T>::Any*>(p);
@@ -42,7 +42,7 @@ __device__ __forceinline__ void mbvae_load_vec(const T* p, int64_t left, float* 
 
 // The same as one vector of the type itself.
 template <typename T>
-__device__ __forceinline__ typename MbvaeVec<T>::Aligned mbvae_load_raw(const T* p, int64_t left) {
+__device__ __forceinline__ typename MbvaeVec<T>::Aligned mbvae_load_raw(const T* p, int left) {
   constexpr int N = MbvaeVec<T>::N;
   typename MbvaeVec<T>::Aligned t;
   if (left >= N) {
@@ -56,7 +56,7 @@ __device__ __forceinline__ typename MbvaeVec<T>::Aligned mbvae_load_raw(const T*
 
 // The first min(N, left) elements at p = v, each rounded once to nearest even.
 template <typename T>
-__device__ __forceinline__ void mbvae_store_vec(T* p, int64_t left, const float* v) {
+__device__ __forceinline__ void mbvae_store_vec(T* p, int left, const float* v) {
   constexpr int N = MbvaeVec<T>::N;
   if (left >= N) {
     typename MbvaeVec<T>::Aligned t;
@@ -71,11 +71,6 @@ __device__ __forceinline__ void mbvae_store_vec(T* p, int64_t left, const float*
 }
 
 // Parameter vectors (gamma, beta, scale) may have another type than the activations: the type is a run-time, wave-uniform choice.
-__device__ __forceinline__ float mbvae_load_param(const void* p, int dtype, int64_t i) {
-  if (dtype == MBVAE_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == MBVAE_BF16) return (float)reinterpret_cast<const mbvae_bf16*>(p)[i];
-  return (float)reinterpret_cast<const mbvae_f16*>(p)[i];
-}
 __device__ __forceinline__ void mbvae_store_param(void* p, int dtype, int64_t i, float v) {
   if (dtype == MBVAE_F32) reinterpret_cast<float*>(p)[i] = v;
   else if (dtype == MBVAE_BF16) reinterpret_cast<mbvae_bf16*>(p)[i] = (mbvae_bf16)v;
