@@ -48,13 +48,21 @@ __global__ __launch_bounds__(256) void gated_norm_sums_kernel(const float* __res
 
 constexpr int MAX_D = 8192;
 
-int64_t blocks_for(int dtype, int64_t rows, int64_t D, int64_t most) {
+// Blocks: as many as keep `waves` waves on every compute unit, at least one.  More of them have more places of memory open at once and
+// were slower: forward over 1 M rows of 64 fp32 values 282 us with 4096 blocks of four waves, 262 with 2048, 246-252 with 768 (12 waves a
+// unit), 287 with 512; backward 452 with 1024, 428 with 768, 410 with 512 (8 waves), 384 with 256 (4 waves) - which in turn is slower
+// where a block has few rows (16 384 rows of 256 bf16 values: 26.3 / 26.0 / 21.5 / 25.2 us).
+int64_t blocks_for(int dtype, int64_t rows, int64_t D, int waves) {
   const GatedNormShape s = gated_norm_shape(dtype, (int)D);
-  const int64_t teams = s.block / s.threads_a_row;
+  const int64_t teams = s.block / s.threads_a_row, most = (int64_t)mbvae_num_cus() * std::max(1, waves / (s.block / 64));
   return std::max<int64_t>(1, std::min<int64_t>((rows + teams - 1) / teams, most));
 }
-int64_t fwd_blocks(int dtype, int64_t rows, int64_t D) { return blocks_for(dtype, rows, D, 2048); }
-int64_t bwd_blocks(int dtype, int64_t rows, int64_t D) { return blocks_for(dtype, rows, D, 1024); }
+int64_t fwd_blocks(int dtype, int64_t rows, int64_t D) { return blocks_for(dtype, rows, D, 12); }
+int64_t bwd_blocks(int dtype, int64_t rows, int64_t D) {
+  const GatedNormShape s = gated_norm_shape(dtype, (int)D);
+  const int64_t walk = rows / (s.block / s.threads_a_row) / mbvae_num_cus();      // rows a team would walk over with one block a unit
+  return blocks_for(dtype, rows, D, walk >= 128 ? 4 : 8);
+}
 
 int check(const GatedNormArgs& a, int dtype, int64_t rows, int64_t D, int ptype) {
   if (rows < 0 || D <= 0 || mbvae_dtype_size(dtype) == 0 || mbvae_dtype_size(ptype) == 0) return MBVAE_EINVAL;

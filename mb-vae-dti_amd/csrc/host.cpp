@@ -143,8 +143,8 @@ struct Embedding : torch::autograd::Function<Embedding> {
     Tensor dw = at::empty({vocab, D}, dy.options().requires_grad(false));
     if (vocab > 0 && D > 0) {
       const Rows d(dy, D);
-      const Tensor ws = bytes_on(dy, lib.embedding_bwd_workspace(rows, vocab, D, type_code(dy.scalar_type())));
       const c10::DeviceGuard guard(dy.device());
+      const Tensor ws = bytes_on(dy, lib.embedding_bwd_workspace(rows, vocab, D, type_code(dy.scalar_type())));
       succeeded(lib.embedding_bwd(ids.const_data_ptr(), id_code(ids.scalar_type()), d.t.const_data_ptr(), d.ld, dw.mutable_data_ptr(), rows, vocab, D,
                                   (float)ctx->saved_data["scale"].toDouble(), type_code(dy.scalar_type()), ws.mutable_data_ptr(), ws.numel(),
                                   stream_of(dy)),
@@ -226,8 +226,8 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     for (int i = 0, edge = 0; i < 8; ++i)                     // (operands that are absent have no edge)
       if (of[i]->defined() && ctx->needs_input_grad(edge++)) out[i] = contiguous_like(*of[i]);
     const int code = type_code(x.scalar_type());
-    const Tensor ws = bytes_on(x, lib.gated_norm_bwd_workspace(rows, D, code));
     const c10::DeviceGuard guard(x.device());
+    const Tensor ws = bytes_on(x, lib.gated_norm_bwd_workspace(rows, D, code));
     succeeded(lib.gated_norm_bwd(ptr(xr.t), xr.ld, ptr(ur.t), ur.ld, ptr(zr.t), zr.ld, (const uint8_t*)ptr(keep),
                                  (float)ctx->saved_data["keep_scale"].toDouble(), ptr(post_g), ptr(post_b), ptr(scale), ptr(pre_g),
                                  stats.data_ptr<float>(), ptr(dyr.t), dyr.ld, ptr(dnr.t), dnr.ld, out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]),
