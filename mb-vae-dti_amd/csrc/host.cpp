@@ -85,6 +85,15 @@ mbvae_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream
 Tensor bytes_on(const Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte).requires_grad(false)); }
 Tensor contiguous_like(const Tensor& t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
 
+// n elements of a flat buffer from `at` on, as a tensor of its own (the gradients of a block's vectors share one allocation: asking the
+// allocator for each of them took longer than the kernel that writes them).
+Tensor part_of(const Tensor& flat, int64_t at, int64_t n) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
+  impl->set_storage_offset(at);
+  impl->set_sizes_contiguous({n});
+  return Tensor(std::move(impl));
+}
+
 void check_typed(const Tensor& t, const char* what, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.layout() == at::kStrided && type_code(t.scalar_type()) >= 0, what, ": ", name,
               ": expected a dense float32, bfloat16 or float16 tensor on the GPU (got ", name_of(t.scalar_type()), " on ", t.device(),
@@ -223,8 +232,19 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     const Rows xr(x, D), ur(u, D), zr(z, D), dyr(dy, D), dnr(dn, D);
     const int64_t rows = xr.t.size(0);
     const Tensor* of[8] = {&x, &u, &z, &post_g, &post_b, &scale, &pre_g, &pre_b};
-    for (int i = 0, edge = 0; i < 8; ++i)                     // (operands that are absent have no edge)
-      if (of[i]->defined() && ctx->needs_input_grad(edge++)) out[i] = contiguous_like(*of[i]);
+    int vectors = 0;
+    bool wanted[8];
+    for (int i = 0, edge = 0; i < 8; ++i) {                   // (operands that are absent have no edge)
+      wanted[i] = of[i]->defined() && ctx->needs_input_grad(edge++);
+      if (wanted[i] && i < 3) out[i] = contiguous_like(x);
+      vectors += wanted[i] && i >= 3;
+    }
+    if (vectors) {
+      const Tensor& any = post_g.defined() ? post_g : scale.defined() ? scale : pre_g;
+      const Tensor flat = at::empty({vectors * D}, any.options().requires_grad(false));
+      for (int i = 3, k = 0; i < 8; ++i)
+        if (wanted[i]) out[i] = part_of(flat, D * k++, D);
+    }
     const int code = type_code(x.scalar_type());
     const c10::DeviceGuard guard(x.device());
     const Tensor ws = bytes_on(x, lib.gated_norm_bwd_workspace(rows, D, code));
