@@ -46,6 +46,32 @@ def _gated(seq, x, u, gate_in, activation, training):
     return ops.gate_update(x, u, z, seq[5].p, training)
 
 
+# ------------------------------------------------------------------------------------------------ fused blocks (ops.set_fused_blocks)
+def _affine(ln):
+    return ln.weight, ln.bias
+
+
+def _step(x, u, z, p, training, following):
+    """(x + u * dropout(sigmoid(z)), LayerNorm `following` of it) in one kernel; u None: x itself is gated, z None: no gate.  Draws the
+    same keep mask as ops.gate_update."""
+    keep, scale = None, 1.0
+    if z is not None and training and p > 0:
+        keep = torch.empty(z.shape, dtype=torch.uint8, device=z.device).bernoulli_(1.0 - p)
+        scale = 1.0 / (1.0 - p)
+    pre, eps = (None, 1e-5) if following is None else (_affine(following), following.eps)
+    return ops.gated_residual_norm(x, u, z, keep=keep, keep_scale=scale, pre=pre, eps=eps)
+
+
+def _mlp_of(seq, n, activation, training):
+    """_mlp_block behind its LayerNorm, whose output n is."""
+    return _lin(seq[4], _drop(_act_linear(seq[1], n, activation), seq[3].p, training))
+
+
+def _gate_of(seq, n, activation):
+    """The gate's logits behind its LayerNorm, whose output n is."""
+    return _lin(seq[3], _act_linear(seq[1], n, activation))
+
+
 class ResidualEncoder(nn.Module):
     """Pre-norm residual MLP encoder."""
 
@@ -61,6 +87,12 @@ class ResidualEncoder(nn.Module):
 
     def forward(self, x):
         x = _lin(self.input_proj, x)
+        if ops.fused_blocks():
+            norms = [blk[0] for blk in self.layers] + [self.output_proj[0]]
+            n = _ln(norms[0], x)
+            for blk, following in zip(self.layers, norms[1:]):
+                x, n = _step(x, _mlp_of(blk, n, self.activation, self.training), None, 0.0, self.training, following)
+            return _lin(self.output_proj[1], n)
         for blk in self.layers:
             x = x + _mlp_block(blk, x, self.activation, self.training)
         return _lin(self.output_proj[1], _ln(self.output_proj[0], x))
@@ -85,6 +117,14 @@ class TransformerEncoder(nn.Module):
 
     def forward(self, x):
         x = _lin(self.input_proj, x)
+        if ops.fused_blocks():
+            act, tr = self.activation, self.training
+            norms = [att[0] for att in self.att_layers] + [self.output_proj[0]]
+            n = _ln(norms[0], x)
+            for att, mlp, following in zip(self.att_layers, self.mlp_layers, norms[1:]):
+                x, n = _step(x, None, _gate_of(att, n, act), att[5].p, tr, mlp[0])
+                x, n = _step(x, _mlp_of(mlp, n, act, tr), None, 0.0, tr, following)
+            return _lin(self.output_proj[1], n)
         for att, mlp in zip(self.att_layers, self.mlp_layers):
             x = _gated(att, x, None, x, self.activation, self.training)
             x = x + _mlp_block(mlp, x, self.activation, self.training)
@@ -156,7 +196,17 @@ class CrossAttentionFusion(nn.Module):
 
     def forward(self, a, b):
         act, tr = self.activation, self.training
-        for i in range(self.n_layers):
+        for i in range(self.n_layers if ops.fused_blocks() else 0):
+            gate_a, gate_b, self_a, self_b = self.cross_gates_b_to_a[i], self.cross_gates_a_to_b[i], self.self_gates_a[i], self.self_gates_b[i]
+            ab, ba = torch.cat([a, b], dim=-1), torch.cat([b, a], dim=-1)
+            ua, ub = _lin(self.align_proj_b_to_a[i], b), _lin(self.align_proj_a_to_b[i], a)
+            a, na = _step(a, ua, _gate_of(gate_a, _ln(gate_a[0], ab), act), gate_a[5].p, tr, self_a[0])
+            b, nb = _step(b, ub, _gate_of(gate_b, _ln(gate_b[0], ba), act), gate_b[5].p, tr, self_b[0])
+            a, na = _step(a, None, _gate_of(self_a, na, act), self_a[5].p, tr, self.mlp_a[i][0])
+            b, nb = _step(b, None, _gate_of(self_b, nb, act), self_b[5].p, tr, self.mlp_b[i][0])
+            a = a + _mlp_of(self.mlp_a[i], na, act, tr)
+            b = b + _mlp_of(self.mlp_b[i], nb, act, tr)
+        for i in range(0 if ops.fused_blocks() else self.n_layers):
             a, b = (_gated(self.cross_gates_b_to_a[i], a, _lin(self.align_proj_b_to_a[i], b), torch.cat([a, b], dim=-1), act, tr),
                     _gated(self.cross_gates_a_to_b[i], b, _lin(self.align_proj_a_to_b[i], a), torch.cat([b, a], dim=-1), act, tr))
             a = _gated(self.self_gates_a[i], a, None, a, act, tr)

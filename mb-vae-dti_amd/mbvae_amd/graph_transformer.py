@@ -357,8 +357,24 @@ class GraphTransformer(nn.Module):
                                        "tile_map": ops.edge_tile_map(node_mask), "order": None, "pack": None}
         return self._padding_shortcuts(node_mask)
 
-    def forward(self, X, E, y, node_mask):
+    def _edge_input_from_classes(self, edge_ids, n_classes):
+        """relu(mlp_in_E(one-hot rows)) from class ids: the MLP runs on the n_classes + 1 different rows there are (the last of
+        them all-zero, for ids that are no class) and its outputs are looked up pair by pair; their gradients meet in the table's."""
+        table = torch.eye(n_classes + 1, n_classes, device=edge_ids.device)
+        for lin in (self.mlp_in_E[0], self.mlp_in_E[2]):
+            table = _lin(lin, table, act=1)
+        return ops.embedding(torch.where((edge_ids >= 0) & (edge_ids < n_classes), edge_ids, n_classes), table)
+
+    def forward(self, X, E, y, node_mask, edge_ids=None):
+        """edge_ids (optional, integers [bs,n,n]): the class of every pair whose row of E is one-hot, anything outside the classes
+        (-1) where the row is all-zero.  The edge input MLP then runs once per class instead of once per pair; E itself is still
+        needed for the skip connection at the output."""
         n = X.shape[1]
+        if edge_ids is not None:
+            if edge_ids.shape != E.shape[:-1] or edge_ids.is_floating_point():
+                raise ValueError(f"edge_ids must be integers of shape {tuple(E.shape[:-1])}, got {edge_ids.dtype} {tuple(edge_ids.shape)}")
+            if edge_ids.dtype != torch.int64 and E.shape[-1] > torch.iinfo(edge_ids.dtype).max:
+                edge_ids = edge_ids.long()                       # (the all-zero row's id has to fit)
         X, E, y = X.float(), E.float(), y.float()
         xm = node_mask.unsqueeze(-1).to(X.dtype)
         seeds = _SeedStream(self.training)
@@ -373,9 +389,13 @@ class GraphTransformer(nn.Module):
             tile_map, order = self._padding_shortcuts(node_mask)
             if order is not None and order.sparse and self.n_layers > 0:
                 pack = self._pad_cache.get("pack")
+        def edge_in():
+            return mlp(self.mlp_in_E, E, True) if edge_ids is None else self._edge_input_from_classes(edge_ids, E.shape[-1])
+
         if pack is not None:            # the edge input MLP on the valid pairs only (sym_mask zeroes the others anyway)
             Eflat = E.reshape(-1, E.shape[-1])
-            hv = mlp(self.mlp_in_E, Eflat[pack.pair_rows], True)
+            hv = (mlp(self.mlp_in_E, Eflat[pack.pair_rows], True) if edge_ids is None
+                  else self._edge_input_from_classes(edge_ids.reshape(-1)[pack.pair_rows], E.shape[-1]))
             hE = hv.new_zeros((Eflat.shape[0], hv.shape[-1])).index_copy_(0, pack.pair_rows, hv)
             hE = ops.sym_mask(hE.reshape(*E.shape[:-1], -1), node_mask)
         # training with a second stream: the node / global input and output MLPs (small) next to the edge ones (long)
@@ -388,12 +408,12 @@ class GraphTransformer(nn.Module):
             with torch.cuda.stream(side):
                 hX = mlp(self.mlp_in_X, X, True, mask=node_mask, mask_mode=ops.MASK_NODE, n_nodes=n)
                 hy = mlp(self.mlp_in_y, y, True)
-            hE = ops.sym_mask(mlp(self.mlp_in_E, E, True), node_mask)
+            hE = ops.sym_mask(edge_in(), node_mask)
             main.wait_stream(side)
             hX.record_stream(main); hy.record_stream(main)
             hX._mbvae_stream = hy._mbvae_stream = side
         elif pack is None:
-            hE = ops.sym_mask(mlp(self.mlp_in_E, E, True), node_mask)
+            hE = ops.sym_mask(edge_in(), node_mask)
         if side is not None:
             pass
         elif pack is not None:

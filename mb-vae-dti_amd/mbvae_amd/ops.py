@@ -29,6 +29,22 @@ def set_bf16_storage(on):
 def bf16_storage():
     return _BF16_STORAGE
 
+
+# Opt-in: the feature encoders and the drug / target fusion run each gate or residual update together with the LayerNorm that
+# opens the next block (gated_residual_norm) instead of as separate kernels.  Same function and the same dropout masks; sums in another
+# order, so results agree to fp32 rounding and not bit for bit.
+_FUSED_BLOCKS = os.environ.get("MBVAE_FUSED_BLOCKS", "0") not in ("", "0")
+
+
+def set_fused_blocks(on):
+    """Switch the fused block updates of the encoders and the fusion on or off (takes effect at the next forward)."""
+    global _FUSED_BLOCKS
+    _FUSED_BLOCKS = bool(on)
+
+
+def fused_blocks():
+    return _FUSED_BLOCKS
+
 _ws_cache = {}
 
 

@@ -42,7 +42,7 @@ def synthetic_graphs(bs, n, device, generator, sizes=None):
 
 class DenoiserTrainStep:
     def __init__(self, cfg=CFG3, T=500, lr=5e-4, weight_decay=1e-4, lambdas=(1.0, 5.0), device="cuda", distributed=False,
-                 seed=0, side_stream=None, overlap_optimizer=False):
+                 seed=0, side_stream=None, overlap_optimizer=False, edge_classes=False, max_grad_norm=None):
         # side_stream: the node / global-feature remainder of every layer on a second HIP stream next to the long edge-tensor
         # kernels (ops.set_side_stream; bit-identical to one stream, tests/test_gpu_two_streams.py).  None = on for a GPU
         # model unless MBVAE_SIDE_STREAM=0; an explicit True / False is never overridden by the environment.  With
@@ -67,6 +67,10 @@ class DenoiserTrainStep:
         # dtype/device group instead of ~10 element-wise passes over the 73 M parameters
         self.opt = torch.optim.AdamW(self.model.parameters(), lr=lr, weight_decay=weight_decay, amsgrad=True,
                                      fused=True)
+        # edge_classes: the edge input MLP once per bond class instead of once per pair (GraphTransformer.forward's edge_ids; same
+        # function, sums in another order).  max_grad_norm: clip the gradients' global 2-norm before the update (ops.clip_grad_norm_,
+        # what Lightning's gradient_clip_val does); the norm is left in last["grad_norm"].
+        self.edge_classes, self.max_grad_norm = edge_classes, max_grad_norm
         self.last = {}
         self._params = [p for p in self.model.parameters() if p.requires_grad]
         self._opt_pending = None
@@ -93,19 +97,24 @@ class DenoiserTrainStep:
         t = t_int / self.T
         abar_t = self.schedule.get_alpha_bar(t_normalized=t)
         eX, eE = exp_draws(bs * n, cx, dev), exp_draws(bs * n * n, ce, dev)
-        _, _, X_t, E_t = ops.apply_noise(X0, E0, mask, abar_t, self.mx, self.me, eX, eE)
+        _, E_class, X_t, E_t = ops.apply_noise(X0, E0, mask, abar_t, self.mx, self.me, eX, eE)
         Xg, yg = self.graph_feats(E_t, mask)
         Xm, ym = self.mol_feats(X_t, E_t, truncate_weight=True)
         X_in = torch.cat((X_t, Xg, Xm), 2)
         y_in = torch.cat((cond, yg, ym, t), 1)
         self.wait_optimizer()                       # the previous step's weight update may still run on the second stream
-        pred = self.model(X_in, E_t, y_in, mask)
+        # (the noised class of a masked or diagonal pair is not in E_t: its row there is all-zero)
+        edge_ids = torch.where(E_t.sum(-1) > 0, E_class, -1) if self.edge_classes else None
+        pred = self.model(X_in, E_t, y_in, mask, edge_ids=edge_ids)
         lX, sX = ops.masked_ce(pred.X, X0)
         lE, sE = ops.masked_ce(pred.E, E0)
         loss = self.lambdas[0] * lX + self.lambdas[1] * lE
         loss.backward()
         if self.sync is not None:
             self.sync.finish()
+        grad_norm = None
+        if self.max_grad_norm is not None:
+            grad_norm = ops.clip_grad_norm_([p.grad for p in self._params], self.max_grad_norm)
         side = ops.side_stream(dev) if self.sync is None else None
         if side is None:
             self.opt.step()
@@ -129,4 +138,6 @@ class DenoiserTrainStep:
         else:
             self.opt.zero_grad(set_to_none=True)
         self.last = {"loss": loss.detach(), "ce_X": sX, "ce_E": sE}
+        if grad_norm is not None:
+            self.last["grad_norm"] = grad_norm
         return loss.detach()

@@ -668,3 +668,171 @@ def test_outputs_end_where_they_end(ops):
             for b in (buf, nbuf):
                 assert bool((b[:guard] == 3).all()) and bool((b[guard + size:] == 3).all())
             assert half_step(dtype) > 0
+
+
+# ------------------------------------------------------------------------------------------------ where the framework uses them
+def _close(a, b, rel, what):
+    """Relative error in the 2-norm."""
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    assert a.shape == b.shape and bool(torch.isfinite(a).all()), what
+    assert float((a - b).norm()) <= rel * float(b.norm()), f"{what}: {float((a - b).norm() / b.norm()):.2e}"
+
+
+@pytest.mark.parametrize("which", ["residual", "transformer", "fusion"])
+@pytest.mark.parametrize("bias,dropout", [(True, 0.0), (True, 0.1), (False, 0.1)])
+def test_fused_blocks_of_the_encoders(ops, which, bias, dropout):
+    """Encoders and fusion with the fused updates against the separate kernels: the same dropout masks from the same generator, outputs and
+    all gradients to fp32 rounding.  The chain is 3 layers of norms, products of up to 256 terms and gates; a rounding of 2^-24 a step grows by
+    the layers' condition, a few hundred steps of it stay below 1e-5 - but for ReLU gates that flip, none of which these inputs have
+    within rounding (checked by the bound itself)."""
+    from mbvae_amd import blocks
+    torch.manual_seed(5)
+    if which == "fusion":
+        net = blocks.CrossAttentionFusion(64, 32, 3, factor=4, dropout=dropout, bias=bias).cuda().train()
+        inputs = [torch.randn(40, 64).cuda().requires_grad_(True) for _ in range(2)]
+    else:
+        cls = blocks.ResidualEncoder if which == "residual" else blocks.TransformerEncoder
+        net = cls(100, 64, 48, 3, factor=4, dropout=dropout, bias=bias).cuda().train()
+        inputs = [torch.randn(40, 100).cuda().requires_grad_(True)]
+    leaves = inputs + list(net.parameters())
+
+    def run(fused):
+        ops.set_fused_blocks(fused)
+        try:
+            torch.manual_seed(6)
+            out = net(*inputs)
+            out = out if torch.is_tensor(out) else out[0]
+            state = torch.cuda.get_rng_state()
+            return out, torch.autograd.grad(out.square().sum(), leaves, allow_unused=True), state
+        finally:
+            ops.set_fused_blocks(False)
+
+    want, wg, ws = run(False)
+    got, gg, gs = run(True)
+    assert torch.equal(ws, gs), "the generator has advanced differently"
+    _close(got, want, 1e-5, "output")
+    names = [f"input {i}" for i in range(len(inputs))] + [k for k, _ in net.named_parameters()]
+    for k, a, b in zip(names, gg, wg):
+        assert (a is None) == (b is None), k
+        if a is not None:
+            _close(a, b, 1e-5, k)
+    net.eval()
+    with torch.no_grad():
+        ops.set_fused_blocks(True)
+        got = net(*inputs)
+        ops.set_fused_blocks(False)
+        want = net(*inputs)
+    for a, b in zip(got if isinstance(got, tuple) else [got], want if isinstance(want, tuple) else [want]):
+        _close(a, b, 1e-5, "evaluation")
+
+
+def _small_denoiser():
+    from mbvae_amd.graph_transformer import GraphTransformer
+    torch.manual_seed(7)
+    return GraphTransformer(n_layers=2, input_dims={"X": 13, "E": 5, "y": 77}, hidden_mlp_dims={"X": 32, "E": 16, "y": 64},
+                            hidden_dims={"dx": 64, "de": 16, "dy": 64, "n_head": 4, "dim_ffX": 32, "dim_ffE": 16, "dim_ffy": 64},
+                            output_dims={"X": 5, "E": 5, "y": 64}).cuda()
+
+
+@pytest.mark.parametrize("id_dtype", [torch.int8, torch.int64])
+def test_denoiser_from_edge_classes(ops, id_dtype):
+    """GraphTransformer.forward with the pairs' classes against the one-hot rows alone: outputs and all gradients to fp32 rounding (the edge
+    input MLP sees the same rows; only the order in which its gradients are summed differs)."""
+    from mbvae_amd.trainstep import synthetic_graphs
+    net = _small_denoiser()
+    g = _gen(8)
+    bs, n = 5, 12
+    X0, E0, mask = synthetic_graphs(bs, n, "cuda", g, sizes=torch.tensor([12, 9, 1, 12, 3]))
+    E0 = E0 * (mask.unsqueeze(1) & mask.unsqueeze(2)).unsqueeze(-1)
+    ids = torch.where(E0.sum(-1) > 0, E0.argmax(-1), -1).to(id_dtype)
+    X, y = torch.cat((X0, torch.randn(bs, n, 8, generator=g).cuda()), 2), torch.randn(bs, 77, generator=g).cuda()
+    w = [torch.randn(*s, generator=g).cuda() for s in ((bs, n, 5), (bs, n, n, 5))]
+
+    def run(**kw):
+        out = net(X, E0, y, mask, **kw)
+        params = [p for k, p in net.named_parameters() if "mlp_out_y" not in k]
+        return out, torch.autograd.grad((out.X * w[0]).sum() + (out.E * w[1]).sum(), params, allow_unused=True)
+
+    for train in (False, True):
+        net.train(train)
+        for layer in net.tf_layers:
+            layer.dropout_p = 0.0                       # (dropout draws from the seeds' order, which is the same; off for the comparison)
+        want, wg = run()
+        got, gg = run(edge_ids=ids)
+        _close(got.X, want.X, 1e-5, "X")
+        _close(got.E, want.E, 1e-5, "E")
+        for (k, _), a, b in zip([(k, p) for k, p in net.named_parameters() if "mlp_out_y" not in k], gg, wg):
+            if b is not None and float(b.norm()) > 1e-4:
+                _close(a, b, 2e-5, k)
+    net.eval()
+    with torch.no_grad():
+        for _ in range(2):                              # (the second call takes the packed path where the widths allow it)
+            want, got = net(X, E0, y, mask), net(X, E0, y, mask, edge_ids=ids)
+            _close(got.E, want.E, 1e-5, "E without gradients")
+    for bad in (ids[..., :-1], ids.float()):
+        with pytest.raises(ValueError, match="edge_ids"):
+            net(X, E0, y, mask, edge_ids=bad)
+
+
+def test_train_step_with_classes_and_clipping(ops):
+    """DenoiserTrainStep with edge_classes and max_grad_norm: the same loss as without, the gradients' norm as torch computes it, and the
+    update of clipped gradients."""
+    from mbvae_amd.trainstep import CFG3, DenoiserTrainStep, synthetic_graphs
+    cfg = {**CFG3, "n_layers": 1, "hidden_mlp_dims": {"X": 32, "E": 16, "y": 64}, "input_dims": {"X": 13, "E": 5, "y": 77}, "output_dims": {"X": 5, "E": 5, "y": 64},
+           "hidden_dims": {"dx": 64, "de": 16, "dy": 64, "n_head": 4, "dim_ffX": 32, "dim_ffE": 16, "dim_ffy": 64}}
+    g = _gen(9)
+    X0, E0, mask = synthetic_graphs(8, 16, "cuda", g, sizes=torch.randint(2, 17, (8,), generator=g))
+    cond = torch.randn(8, 64, generator=g).cuda()
+
+    def run(**kw):
+        step = DenoiserTrainStep(cfg=cfg, side_stream=False, **kw)
+        for layer in step.model.tf_layers:
+            layer.dropout_p = 0.0
+        taken = []
+        update = step.opt.step
+
+        def spy(*a, **k):
+            taken.append([p.grad.clone() for p in step.model.parameters() if p.grad is not None])
+            return update(*a, **k)
+
+        step.opt.step = spy
+        torch.manual_seed(10)
+        loss = step.step(X0, E0, mask, cond)
+        return loss, taken[0], step.last
+
+    loss, grads, last = run()
+    assert "grad_norm" not in last
+    total = torch.linalg.vector_norm(torch.cat([t.double().reshape(-1) for t in grads]))
+    for kw in (dict(max_grad_norm=0.1 * float(total)), dict(edge_classes=True, max_grad_norm=0.1 * float(total))):
+        l2, g2, last = run(**kw)
+        _close(l2, loss, 1e-6, "loss")
+        _close(last["grad_norm"], total, 2e-5, "norm")
+        _close(torch.linalg.vector_norm(torch.cat([t.double().reshape(-1) for t in g2])), 0.1 * total, 2e-5, "clipped norm")
+
+
+def test_lightning_gradient_clipping_hook(ops):
+    from mbvae_amd.abstract import AbstractDTIModel
+    model = AbstractDTIModel()
+    model.lin = torch.nn.Linear(8, 4).cuda()
+    model.unused = torch.nn.Parameter(torch.zeros(3).cuda())
+    opt = torch.optim.SGD(model.parameters(), lr=0.1)
+
+    def grads():
+        opt.zero_grad()
+        (model.lin(torch.ones(5, 8, device="cuda")).sum() * 3).backward()
+        return [p.grad for p in model.lin.parameters()]
+
+    before = [t.clone() for t in grads()]
+    norm = torch.cat([t.reshape(-1) for t in before]).double().norm()
+    model.configure_gradient_clipping(opt, None)
+    model.configure_gradient_clipping(opt, 0.0, "norm")
+    assert all(torch.equal(a, p.grad) for a, p in zip(before, model.lin.parameters())) and "train/grad_norm" not in model.logged
+    model.configure_gradient_clipping(opt, 0.5)
+    for a, p in zip(before, model.lin.parameters()):
+        check(p.grad, a.double() * (0.5 / (norm + 1e-6)), (a.double() * 0.5 / norm).abs() * 4 * U, "clipped by norm")
+    check(model.logged["train/grad_norm"], norm, float(norm) * 2 * U, "logged norm")
+    grads()
+    model.configure_gradient_clipping(opt, 2.0, "value")
+    assert all(float(p.grad.abs().max()) <= 2.0 for p in model.lin.parameters())
+    with pytest.raises(ValueError, match="gradient_clip_algorithm"):
+        model.configure_gradient_clipping(opt, 1.0, "other")
