@@ -206,7 +206,8 @@ __device__ __forceinline__ void fill_zero_any(void* p, int dtype, int64_t values
 // Block b puts the tokens with keys in [b * range, (b + 1) * range) in order (range <= 256) and clears the gradient rows of its keys
 // that no token has.  Every wave scans a 16th of all tokens; its finds (place | local key << 16) go to its own part of the list.
 constexpr int ORDER_TOKENS = 32768;             // list entries: 128 KB of LDS, places fit 16 bits
-constexpr int ORDER_BLOCKS = 256;
+constexpr int ORDER_BLOCKS = 256;               // of a table of up to 65 536 rows; larger ones take blocks of 256 rows each
+constexpr int64_t ORDER_VOCAB = (int64_t)1 << 18;
 constexpr int ORDER_COUNTERS = SORT_WAVES * RADIX + 2 * RADIX + SORT_WAVES;
 static_assert(4 * (ORDER_TOKENS + ORDER_COUNTERS) <= MBVAE_LDS_LIMIT, "LDS of one block");
 
@@ -562,7 +563,7 @@ Plan plan_for(int64_t rows, int64_t V, int64_t D, int dtype) {
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   p.lanes = lanes_for((D + vec_of(dtype) - 1) / vec_of(dtype), 64);
-  p.route = V * vec_of(dtype) <= FEW_CELLS ? FEW_CLASSES : rows <= ORDER_TOKENS && V < RADIX * ORDER_BLOCKS ? FEW_TOKENS : RADIX_SORT;
+  p.route = V * vec_of(dtype) <= FEW_CELLS ? FEW_CLASSES : rows <= ORDER_TOKENS && V < ORDER_VOCAB ? FEW_TOKENS : RADIX_SORT;
   if (p.route == FEW_CLASSES) {
     const int64_t teams = 256 / p.lanes;
     p.blocks = std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS, (rows + 8 * teams - 1) / (8 * teams)));
@@ -631,7 +632,7 @@ int launch_bwd(const Plan& p, const void* ids, int id_type, const T* dy, int64_t
     return mbvae_launch_status();
   }
   if (p.route == FEW_TOKENS) {
-    const int64_t range = (V + ORDER_BLOCKS) / ORDER_BLOCKS;          // keys 0..V shared out over at most ORDER_BLOCKS blocks
+    const int64_t range = std::min<int64_t>((V + ORDER_BLOCKS) / ORDER_BLOCKS, RADIX);          // keys 0..V shared out over the blocks
     const int span = (int)((rows + 64 * SORT_WAVES - 1) / (64 * SORT_WAVES)) * 64;
     if (!MBVAE_ALLOW_BIG_LDS(embedding_order_kernel<T>)) return MBVAE_ELAUNCH;
     hipLaunchKernelGGL((embedding_order_kernel<T>), dim3((unsigned)((V + range) / range)), dim3(SORT_THREADS),

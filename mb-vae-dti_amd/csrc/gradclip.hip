@@ -221,7 +221,7 @@ __global__ __launch_bounds__(THREADS) void grad_scale_kernel(Table t, uint32_t c
   const double a = join_partials<P>(part, parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)a;
   const double c = max_norm / (a + 1e-6);
-  const float f = c > 1. ? 1.f : (float)c;                 // (a NaN norm makes every gradient NaN)
+  const float f = c > 1. || max_norm == INFINITY ? 1.f : (float)c;        // (a NaN norm makes every gradient NaN)
   if (in_place && f == 1.f) return;                        // nothing to scale: the values stay as they are
   walk_back(t, share_begin(chunks, blockIdx.x, gridDim.x), share_begin(chunks, blockIdx.x + 1, gridDim.x), [&](int i, int64_t at, int64_t n) {
     const int dtype = t.last(i) >> 24;

@@ -338,14 +338,14 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
       dst[i] = g.mutable_data_ptr();
     }
   }
+  if (write)                                                 // (refused for tensors that may not be written here, so before the launch)
+    for (const Tensor& t : apart ? out : grads) t.unsafeGetTensorImpl()->bump_version();
   Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
   const Tensor ws = bytes_on(grads[0], lib.grad_clip_workspace((int64_t)count));
   const c10::DeviceGuard guard(device);
   succeeded(lib.grad_clip(src.data(), write ? dst.data() : nullptr, numel.data(), types.data(), (int64_t)count, p, max_norm, norm.data_ptr<float>(),
                           ws.mutable_data_ptr(), ws.numel(), stream_of(grads[0])),
             "mbvae_grad_clip");
-  if (write)
-    for (const Tensor& t : apart ? out : grads) t.unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 

@@ -371,7 +371,7 @@ class GraphTransformer(nn.Module):
         needed for the skip connection at the output."""
         n = X.shape[1]
         if edge_ids is not None:
-            if edge_ids.shape != E.shape[:-1] or edge_ids.is_floating_point():
+            if edge_ids.shape != E.shape[:-1] or edge_ids.is_floating_point() or edge_ids.dtype == torch.bool:
                 raise ValueError(f"edge_ids must be integers of shape {tuple(E.shape[:-1])}, got {edge_ids.dtype} {tuple(edge_ids.shape)}")
             if edge_ids.dtype != torch.int64 and E.shape[-1] > torch.iinfo(edge_ids.dtype).max:
                 edge_ids = edge_ids.long()                       # (the all-zero row's id has to fit)

@@ -1163,8 +1163,8 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, out=None):
     """Scales a list of gradients (p.grad of a model's parameters; None entries are skipped) by min(1, max_norm / (norm + 1e-6)) and
     returns their norm before it as one float32 value on the GPU: what Lightning's gradient_clip_val does (mb_vae_dti/training/run.py:638-654).
     In place, or into `out`: as many tensors of the same types and layouts.  float32, bfloat16 and float16 may be mixed.  Where the norm
-    is within max_norm the values stay bit for bit; a norm of infinity scales by 0, a NaN norm makes every gradient NaN.  No tensor may
-    share memory with another one that is written."""
+    is within max_norm, or max_norm is infinity, the values stay bit for bit; a norm of infinity scales by 0, a NaN norm makes every gradient
+    NaN.  No tensor may share memory with another one that is written."""
     grads, outs = list(grads), None if out is None else list(out)
     if outs is not None and len(outs) != len(grads):
         raise ValueError(f"clip_grad_norm_: {len(grads)} gradients, but {len(outs)} outputs")

@@ -55,7 +55,8 @@ EMBEDDING = [
     (70001, 66000, 20, F32, torch.int64, "hot"), (30000, 9, 1037, BF16, torch.int8, "uniform"), (16385, 11, 8, F32, torch.int8, "none"),
     (17, 20, 2050, F32, torch.int64, "uniform"), (700, 32, 260, F32, torch.int8, "hot"), (700, 33, 260, F32, torch.int8, "hot"), (3000, 16, 520, BF16, torch.int16, "uniform"),
     (3000, 17, 520, BF16, torch.uint8, "hot"), (32768, 4000, 16, F32, torch.int64, "hot"), (32769, 4000, 16, F32, torch.int64, "hot"), (32768, 33, 8, F16, torch.int8, "one"),
-    (900, 65535, 8, F32, torch.int32, "uniform"), (900, 65536, 8, F32, torch.int64, "uniform"), (2, 65000, 4, BF16, torch.int64, "uniform"), (5000, 1, 40, F32, torch.int64, "uniform"),
+    (900, 65535, 8, F32, torch.int32, "uniform"), (900, 65536, 8, F32, torch.int64, "uniform"),
+    (5000, 128000, 8, F32, torch.int64, "uniform"), (9000, 262143, 4, BF16, torch.int32, "hot"), (900, 262144, 4, F32, torch.int64, "sorted"), (33000, 128000, 4, F16, torch.int64, "hot"), (2, 65000, 4, BF16, torch.int64, "uniform"), (5000, 1, 40, F32, torch.int64, "uniform"),
 ]
 
 
@@ -509,6 +510,15 @@ def test_clip_grad_norm_layouts_and_lists(ops):
     assert float(ops.clip_grad_norm_([torch.zeros(0, device="cuda")], 1.0)) == 0
     zero = torch.zeros(100, device="cuda")
     assert float(ops.clip_grad_norm_([zero], 1.0)) == 0 and not bool(zero.any())
+    kept = turned4.clone()
+    with torch.inference_mode():
+        frozen = torch.ones(5, device="cuda")
+    with pytest.raises(RuntimeError, match="nference"):
+        ops.clip_grad_norm_([turned4, frozen], 1e-3)
+    assert torch.equal(turned4, kept)
+    kept[0, 0, 0, 0] = math.inf
+    before = kept.clone()
+    assert float(ops.clip_grad_norm_([kept], math.inf)) == math.inf and torch.equal(kept, before)
     ops.clip_grad_norm_([turned], 0.0)
     assert not bool(turned.any())
 
@@ -769,7 +779,7 @@ def test_denoiser_from_edge_classes(ops, id_dtype):
         for _ in range(2):                              # (the second call takes the packed path where the widths allow it)
             want, got = net(X, E0, y, mask), net(X, E0, y, mask, edge_ids=ids)
             _close(got.E, want.E, 1e-5, "E without gradients")
-    for bad in (ids[..., :-1], ids.float()):
+    for bad in (ids[..., :-1], ids.float(), ids > 0):
         with pytest.raises(ValueError, match="edge_ids"):
             net(X, E0, y, mask, edge_ids=bad)
 
