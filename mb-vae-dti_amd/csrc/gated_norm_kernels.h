@@ -61,12 +61,15 @@ struct Row {
   __device__ __forceinline__ int col(int v) const { return (v * width + lane) * N; }
   __device__ __forceinline__ bool inside(int e) const { return ALIGNED ? col(e / N) < D : col(e / N) + e % N < D; }
 
-  // `on`: whether the row is there at all (a team behind the last row has zeros for all it loads)
-  __device__ __forceinline__ void load(const void* p, int64_t at, bool on, Piece* out) const {
+  // Where the lane's elements of row r begin in an operand with rows ld elements apart; the kernels move these on from row to row.
+  template <typename P>
+  __device__ __forceinline__ P* at(P* p, int64_t r, int64_t ld) const { return p + r * ld + lane * N; }
+  // p: the lane's place in the row.  `on`: whether the row is there at all (a team behind the last row has zeros for all it loads)
+  __device__ __forceinline__ void load(const T* p, bool on, Piece* out) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = col(v), left = on ? D - c : 0;
-      const T* q = reinterpret_cast<const T*>(p) + at + c;
+      const int left = on ? D - col(v) : 0;
+      const T* q = p + v * width * N;
       if (ALIGNED) {
         Piece t = {};
         if (left > 0) t = *reinterpret_cast<const typename MbvaeVec<T>::Any*>(q);
@@ -80,11 +83,11 @@ struct Row {
 #pragma unroll
     for (int e = 0; e < EPL; ++e) out[e] = (float)in[e / N][e % N];
   }
-  __device__ __forceinline__ void store(void* p, int64_t at, bool on, const float* val) const {
+  __device__ __forceinline__ void store(T* p, bool on, const float* val) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = col(v), left = on ? D - c : 0;
-      T* q = reinterpret_cast<T*>(p) + at + c;
+      const int left = on ? D - col(v) : 0;
+      T* q = p + v * width * N;
       if (ALIGNED) {
         if (left > 0) mbvae_store_vec<T>(q, N, val + v * N);
       } else {
@@ -121,16 +124,17 @@ struct Row {
   }
   typedef uint8_t Bytes __attribute__((ext_vector_type(MbvaeVec<T>::N)));
   typedef Bytes AnyBytes __attribute__((aligned(1)));
-  __device__ __forceinline__ void keep(const uint8_t* p, int64_t at, bool on, Bytes* out) const {
+  __device__ __forceinline__ void keep(const uint8_t* p, bool on, Bytes* out) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int c = col(v), left = on ? D - c : 0;
+      const int left = on ? D - col(v) : 0;
+      const uint8_t* q = p + v * width * N;
       Bytes b = {};
-      if (left >= N) b = *reinterpret_cast<const AnyBytes*>(p + at + c);
+      if (left >= N) b = *reinterpret_cast<const AnyBytes*>(q);
       else if (!ALIGNED)
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (e < left) b[e] = p[at + c + e];
+          if (e < left) b[e] = q[e];
       out[v] = b;
     }
   }
@@ -152,7 +156,9 @@ __device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float
     const float d = row.inside(e) ? t[e] - mean : 0.f;
     q = fmaf(d, d, q);
   }
-  r = 1.f / sqrtf(fmaf(team.sum(q), inv_D, eps));
+  // 1 / sqrt(a) to within a rounding: the hardware's and one Newton step (none where that is not finite: eps = 0 and a row of zeros)
+  const float a = fmaf(team.sum(q), inv_D, eps), r0 = __builtin_amdgcn_rsqf(a), step = fmaf(r0 * -a, r0, 1.f);
+  r = a > 1e-37f ? fmaf(0.5f * r0, step, r0) : 1.f / sqrtf(a);
 }
 
 // Both kernels walk over the rows with a fixed grid and ask for the next row's operands before the current row's results are stored: a
@@ -173,19 +179,24 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
   row.param(a.scale, a.ptype, 1.f, sc);
   const int64_t stride = (int64_t)gridDim.x * TEAMS;
   int64_t base = (int64_t)blockIdx.x * TEAMS, r = base + (TPR ? threadIdx.x / (TPR ? TPR : 1) : 0);
+  const T *px = row.at(reinterpret_cast<const T*>(a.x), r, a.ldx), *pu = row.at(reinterpret_cast<const T*>(a.u), r, a.ldu),
+          *pz = row.at(reinterpret_cast<const T*>(a.z), r, a.ldz);
+  const uint8_t* pk = row.at(a.keep, r, a.D);
+  T *py = row.at(reinterpret_cast<T*>(a.y), r, a.D), *pn = row.at(reinterpret_cast<T*>(a.n), r, a.D);
   typename R::Piece xn[NV], un[NV], zn[NV];
   typename R::Bytes kn[NV];
   const auto ask = [&]() {
     const bool on = r < a.rows;
-    row.load(a.x, r * a.ldx, on, xn);
-    if (a.u) row.load(a.u, r * a.ldu, on, un);
-    if (a.z) row.load(a.z, r * a.ldz, on, zn);
-    if (a.keep) row.keep(a.keep, r * a.D, on, kn);
+    row.load(px, on, xn);
+    if (a.u) row.load(pu, on, un);
+    if (a.z) row.load(pz, on, zn);
+    if (a.keep) row.keep(pk, on, kn);
+    px += stride * a.ldx; pu += stride * a.ldu; pz += stride * a.ldz; pk += stride * a.D;
   };
   ask();
   for (; base < a.rows; base += stride) {
     const bool on = r < a.rows;
-    const int64_t at = r * a.D, mine = r;
+    const int64_t mine = r;
     float y[EPL], v[EPL], w[EPL];
     R::widen(xn, y);
     if (a.u) R::widen(un, v);
@@ -219,12 +230,14 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
 #pragma unroll
       for (int e = 0; e < EPL; ++e) y[e] = fmaf(v[e] * w[e], sc[e], y[e]);
     }
-    row.store(a.y, at, on, y);
+    row.store(py, on, y);
+    py += stride * a.D;
     if (a.pre_g) {
       row_stats<EPL>(row, team, y, inv_D, a.rms, a.eps, st.z, st.w);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) y[e] = fmaf((y[e] - st.z) * st.w, ng[e], nb[e]);
-      row.store(a.n, at, on, y);
+      row.store(pn, on, y);
+      pn += stride * a.D;
     }
     if (a.stats && on && row.lane == 0) a.stats[mine] = st;
   }
@@ -258,17 +271,17 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
   const auto ask = [&]() {
     const bool on = r < a.rows;
     sn = on ? a.stats[r] : make_float4(0.f, 0.f, 0.f, 0.f);
-    row.load(a.x, r * a.ldx, on, xn);
-    if (a.u) row.load(a.u, r * a.ldu, on, un);
-    if (a.z) row.load(a.z, r * a.ldz, on, zn);
-    if (a.dy) row.load(a.dy, r * a.lddy, on, tn);
-    if (pre) row.load(a.dn, r * a.lddn, on, dn);
-    if (a.keep) row.keep(a.keep, r * a.D, on, kn);
+    row.load(row.at(reinterpret_cast<const T*>(a.x), r, a.ldx), on, xn);
+    if (a.u) row.load(row.at(reinterpret_cast<const T*>(a.u), r, a.ldu), on, un);
+    if (a.z) row.load(row.at(reinterpret_cast<const T*>(a.z), r, a.ldz), on, zn);
+    if (a.dy) row.load(row.at(reinterpret_cast<const T*>(a.dy), r, a.lddy), on, tn);
+    if (pre) row.load(row.at(reinterpret_cast<const T*>(a.dn), r, a.lddn), on, dn);
+    if (a.keep) row.keep(row.at(a.keep, r, a.D), on, kn);
   };
   if (base < a.rows) ask();
   for (; base < a.rows; base += stride) {
     const bool on = r < a.rows;
-    const int64_t at = r * a.D;
+    const int64_t mine = r;
     const float4 st = sn;
     float x[EPL], v[EPL], w[EPL], dw[EPL], t[EPL], d[EPL];
     R::widen(xn, x);
@@ -328,7 +341,7 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
         sums[GATED_SUM_POST_B][e] += dv[e];
       }
     }
-    if (a.dz) row.store(a.dz, at, on, dw);
+    if (a.dz) row.store(row.at(reinterpret_cast<T*>(a.dz), mine, a.D), on, dw);
     if (post) {
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -343,12 +356,12 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
       for (int e = 0; e < EPL; ++e) dv[e] = st.y * (dv[e] - fmaf(v[e], m2, m1));
     }
     if (a.u) {
-      if (a.du) row.store(a.du, at, on, dv);
+      if (a.du) row.store(row.at(reinterpret_cast<T*>(a.du), mine, a.D), on, dv);
     } else {
 #pragma unroll
       for (int e = 0; e < EPL; ++e) t[e] += dv[e];
     }
-    if (a.dx) row.store(a.dx, at, on, t);
+    if (a.dx) row.store(row.at(reinterpret_cast<T*>(a.dx), mine, a.D), on, t);
   }
   // column sums of the block: its teams in order
   float* part = a.part + (int64_t)blockIdx.x * GATED_SUMS * a.D;
