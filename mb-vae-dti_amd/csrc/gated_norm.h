@@ -20,13 +20,15 @@ struct GatedNormArgs {
   float* part;                        // [blocks][GATED_SUMS][D]
 };
 
-// Threads a row and elements a thread.  Up to 64 pieces of 16 bytes (fp32: up to 512 values) a row belongs to 16, 32 or 64 lanes of a
+// Threads a row and elements a thread.  Up to 64 pieces of 16 bytes (fp32: up to 512 values) a row belongs to 4 to 64 lanes of a
 // wave; wider rows to a block of their own with 8 elements a thread, as few waves as hold the row.
 struct GatedNormShape {
   int threads_a_row, elements, block;
 };
 inline GatedNormShape gated_norm_shape(int dtype, int D) {
   const int N = dtype == MBVAE_F32 ? 4 : 8;
+  if (D <= 4 * N) return {4, N, 256};
+  if (D <= 8 * N) return {8, N, 256};
   if (D <= 16 * N) return {16, N, 256};
   if (D <= 32 * N) return {32, N, 256};
   if (D <= 64 * N) return {64, N, 256};

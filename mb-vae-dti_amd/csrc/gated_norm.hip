@@ -61,7 +61,7 @@ int64_t fwd_blocks(int dtype, int64_t rows, int64_t D) { return blocks_for(dtype
 int64_t bwd_blocks(int dtype, int64_t rows, int64_t D) {
   const GatedNormShape s = gated_norm_shape(dtype, (int)D);
   const int64_t walk = rows / (s.block / s.threads_a_row) / mbvae_num_cus();      // rows a team would walk over with one block a unit
-  return blocks_for(dtype, rows, D, walk >= 128 ? 4 : 8);
+  return blocks_for(dtype, rows, D, walk >= 128 && s.threads_a_row <= 64 ? 4 : 8);
 }
 
 int check(const GatedNormArgs& a, int dtype, int64_t rows, int64_t D, int ptype) {

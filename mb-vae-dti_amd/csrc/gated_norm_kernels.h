@@ -6,7 +6,7 @@
 namespace {
 
 // ------------------------------------------------------------------------------------------------ sums over a row
-// TPR lanes of a wave own a row (16, 32, 64), or, with TPR == 0, a whole block does: its waves meet in LDS, in buffers that alternate so
+// TPR lanes of a wave own a row (4 to 64), or, with TPR == 0, a whole block does: its waves meet in LDS, in buffers that alternate so
 // that one barrier a sum is enough.
 template <int TPR>
 struct Team {
@@ -49,34 +49,44 @@ __device__ __forceinline__ void sigmoid(float z, float& s, float& ds) {
 }
 
 // ------------------------------------------------------------------------------------------------ one thread's elements of a row
-// EPL of them in 16-byte pieces; piece v of thread l begins at column (v * width + l) * N.  ALIGNED: the row is a whole number of
-// pieces, so that a piece is inside it or not; otherwise the last piece is taken element by element.
-template <typename T, int TPR, int EPL, bool ALIGNED>
+// EPL of them in 16-byte pieces; piece v of thread l is the row's (v * width + l)-th.  WHOLE: the row is a whole number of pieces.
+// MOVED: it is not, and its last piece is moved back to end where the row ends: it repeats columns of the piece before, which both
+// threads compute alike and store alike, and which `own` leaves out of the sums.  (Taking the last piece element by element instead made a
+// row of 38 bf16 values 2.4 times as slow.)  SHORT: the row is shorter than one piece and goes element by element.
+enum { WHOLE, MOVED, SHORT };
+template <typename T, int TPR, int EPL, int KIND>
 struct Row {
   static constexpr int N = MbvaeVec<T>::N, NV = EPL / N;
+  static constexpr bool ALIGNED = KIND == WHOLE;
   static_assert(NV * N == EPL, "whole pieces");
   typedef typename MbvaeVec<T>::Aligned Piece;
-  int lane, width, D;
-  __device__ __forceinline__ Row(int columns) : lane(TPR ? threadIdx.x % (TPR ? TPR : 1) : threadIdx.x), width(TPR ? TPR : blockDim.x), D(columns) {}
-  __device__ __forceinline__ int col(int v) const { return (v * width + lane) * N; }
-  __device__ __forceinline__ bool inside(int e) const { return ALIGNED ? col(e / N) < D : col(e / N) + e % N < D; }
+  int lane, D, first[NV], start[NV];              // piece v: the column it is there for, and the one it begins at
+  bool there[NV];
+  __device__ __forceinline__ Row(int columns) : lane(TPR ? threadIdx.x % (TPR ? TPR : 1) : threadIdx.x), D(columns) {
+    const int width = TPR ? TPR : blockDim.x;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      first[v] = (v * width + lane) * N;
+      there[v] = first[v] < D;
+      start[v] = ALIGNED || first[v] + N <= D ? first[v] : KIND == MOVED ? D - N : 0;
+    }
+  }
+  __device__ __forceinline__ int col(int e) const { return start[e / N] + e % N; }
+  // whether element e is one of the row's, and this thread's to count
+  __device__ __forceinline__ bool own(int e) const { return there[e / N] && (ALIGNED || (col(e) >= first[e / N] && col(e) < D)); }
+  __device__ __forceinline__ float counted(int e, float t) const { return ALIGNED || own(e) ? t : 0.f; }
 
-  // Where the lane's elements of row r begin in an operand with rows ld elements apart; the kernels move these on from row to row.
-  template <typename P>
-  __device__ __forceinline__ P* at(P* p, int64_t r, int64_t ld) const { return p + r * ld + lane * N; }
-  // p: the lane's place in the row.  `on`: whether the row is there at all (a team behind the last row has zeros for all it loads)
+  // p: the row.  `on`: whether the row is there at all (a team behind the last row has zeros for all it loads)
   __device__ __forceinline__ void load(const T* p, bool on, Piece* out) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int left = on ? D - col(v) : 0;
-      const T* q = p + v * width * N;
-      if (ALIGNED) {
-        Piece t = {};
-        if (left > 0) t = *reinterpret_cast<const typename MbvaeVec<T>::Any*>(q);
-        out[v] = t;
+      Piece t = {};
+      if constexpr (KIND != SHORT) {
+        if (on && there[v]) t = *reinterpret_cast<const typename MbvaeVec<T>::Any*>(p + start[v]);
       } else {
-        out[v] = mbvae_load_raw<T>(q, left);
+        t = mbvae_load_raw<T>(p, on && there[v] ? D : 0);
       }
+      out[v] = t;
     }
   }
   static __device__ __forceinline__ void widen(const Piece* in, float* out) {
@@ -86,32 +96,26 @@ struct Row {
   __device__ __forceinline__ void store(T* p, bool on, const float* val) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int left = on ? D - col(v) : 0;
-      T* q = p + v * width * N;
-      if (ALIGNED) {
-        if (left > 0) mbvae_store_vec<T>(q, N, val + v * N);
+      if constexpr (KIND != SHORT) {
+        if (on && there[v]) mbvae_store_vec<T>(p + start[v], N, val + v * N);
       } else {
-        mbvae_store_vec<T>(q, left, val + v * N);
+        mbvae_store_vec<T>(p, on && there[v] ? D : 0, val);
       }
     }
   }
   // a vector over the columns in the parameters' type; `none` where p is null
   template <typename P>
   __device__ __forceinline__ void param_of(const P* p, float* out) const {
+    constexpr int M = MbvaeVec<P>::N, STEP = N < M ? N : M;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int q = 0; q < N; q += (N < MbvaeVec<P>::N ? N : MbvaeVec<P>::N)) {
-        constexpr int M = MbvaeVec<P>::N;
-        const int c = col(v) + q;
-        if constexpr (M <= N) {
-          mbvae_load_vec<P>(p + c, D - c, out + v * N + q);
-        } else {
-          float t[M];
-          mbvae_load_vec<P>(p + c, D - c < N ? D - c : N, t);            // (N of a longer piece)
+      for (int q = 0; q < N; q += STEP) {
+        const int left = there[v] ? D - start[v] - q : 0;
+        float t[M];
+        mbvae_load_vec<P>(p + start[v] + q, M > N && left > N ? N : left, t);            // (N of a longer piece)
 #pragma unroll
-          for (int e = 0; e < N; ++e) out[v * N + q + e] = t[e];
-        }
+        for (int e = 0; e < STEP; ++e) out[v * N + q + e] = t[e];
       }
   }
   __device__ __forceinline__ void param(const void* p, int type, float none, float* out) const {
@@ -127,14 +131,14 @@ struct Row {
   __device__ __forceinline__ void keep(const uint8_t* p, bool on, Bytes* out) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int left = on ? D - col(v) : 0;
-      const uint8_t* q = p + v * width * N;
       Bytes b = {};
-      if (left >= N) b = *reinterpret_cast<const AnyBytes*>(q);
-      else if (!ALIGNED)
+      if constexpr (KIND != SHORT) {
+        if (on && there[v]) b = *reinterpret_cast<const AnyBytes*>(p + start[v]);
+      } else if (on && there[v]) {
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (e < left) b[e] = q[e];
+          if (e < D) b[e] = p[e];
+      }
       out[v] = b;
     }
   }
@@ -147,13 +151,13 @@ __device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float
   if (!rms) {
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) s += t[e];
+    for (int e = 0; e < EPL; ++e) s += row.counted(e, t[e]);
     mean = team.sum(s) * inv_D;
   }
   float q = 0.f;
 #pragma unroll
   for (int e = 0; e < EPL; ++e) {
-    const float d = row.inside(e) ? t[e] - mean : 0.f;
+    const float d = row.own(e) ? t[e] - mean : 0.f;
     q = fmaf(d, d, q);
   }
   // 1 / sqrt(a) to within a rounding: the hardware's and one Newton step (none where that is not finite: eps = 0 and a row of zeros)
@@ -163,9 +167,9 @@ __device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float
 
 // Both kernels walk over the rows with a fixed grid and ask for the next row's operands before the current row's results are stored: a
 // load behind a store would wait for it (one counter, in order).
-template <typename T, int TPR, int EPL, int THREADS, bool ALIGNED>
+template <typename T, int TPR, int EPL, int THREADS, int KIND>
 __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a) {
-  typedef Row<T, TPR, EPL, ALIGNED> R;
+  typedef Row<T, TPR, EPL, KIND> R;
   constexpr int TEAMS = TPR ? THREADS / (TPR ? TPR : 1) : 1, NV = R::NV;
   __shared__ float2 red[32];
   Team<TPR> team{red, 0};
@@ -179,10 +183,10 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
   row.param(a.scale, a.ptype, 1.f, sc);
   const int64_t stride = (int64_t)gridDim.x * TEAMS;
   int64_t base = (int64_t)blockIdx.x * TEAMS, r = base + (TPR ? threadIdx.x / (TPR ? TPR : 1) : 0);
-  const T *px = row.at(reinterpret_cast<const T*>(a.x), r, a.ldx), *pu = row.at(reinterpret_cast<const T*>(a.u), r, a.ldu),
-          *pz = row.at(reinterpret_cast<const T*>(a.z), r, a.ldz);
-  const uint8_t* pk = row.at(a.keep, r, a.D);
-  T *py = row.at(reinterpret_cast<T*>(a.y), r, a.D), *pn = row.at(reinterpret_cast<T*>(a.n), r, a.D);
+  const T *px = reinterpret_cast<const T*>(a.x) + r * a.ldx, *pu = reinterpret_cast<const T*>(a.u) + r * a.ldu,
+          *pz = reinterpret_cast<const T*>(a.z) + r * a.ldz;
+  const uint8_t* pk = a.keep + r * a.D;
+  T *py = reinterpret_cast<T*>(a.y) + r * a.D, *pn = reinterpret_cast<T*>(a.n) + r * a.D;
   typename R::Piece xn[NV], un[NV], zn[NV];
   typename R::Bytes kn[NV];
   const auto ask = [&]() {
@@ -243,9 +247,9 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
   }
 }
 
-template <typename T, int TPR, int EPL, int THREADS, bool ALIGNED>
+template <typename T, int TPR, int EPL, int THREADS, int KIND>
 __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a) {
-  typedef Row<T, TPR, EPL, ALIGNED> R;
+  typedef Row<T, TPR, EPL, KIND> R;
   constexpr int TEAMS = TPR ? THREADS / (TPR ? TPR : 1) : 1, NV = R::NV;
   __shared__ float2 red[32];
   __shared__ float join[TEAMS > 1 ? THREADS * EPL : 1];
@@ -271,12 +275,12 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
   const auto ask = [&]() {
     const bool on = r < a.rows;
     sn = on ? a.stats[r] : make_float4(0.f, 0.f, 0.f, 0.f);
-    row.load(row.at(reinterpret_cast<const T*>(a.x), r, a.ldx), on, xn);
-    if (a.u) row.load(row.at(reinterpret_cast<const T*>(a.u), r, a.ldu), on, un);
-    if (a.z) row.load(row.at(reinterpret_cast<const T*>(a.z), r, a.ldz), on, zn);
-    if (a.dy) row.load(row.at(reinterpret_cast<const T*>(a.dy), r, a.lddy), on, tn);
-    if (pre) row.load(row.at(reinterpret_cast<const T*>(a.dn), r, a.lddn), on, dn);
-    if (a.keep) row.keep(row.at(a.keep, r, a.D), on, kn);
+    row.load(reinterpret_cast<const T*>(a.x) + r * a.ldx, on, xn);
+    if (a.u) row.load(reinterpret_cast<const T*>(a.u) + r * a.ldu, on, un);
+    if (a.z) row.load(reinterpret_cast<const T*>(a.z) + r * a.ldz, on, zn);
+    if (a.dy) row.load(reinterpret_cast<const T*>(a.dy) + r * a.lddy, on, tn);
+    if (pre) row.load(reinterpret_cast<const T*>(a.dn) + r * a.lddn, on, dn);
+    if (a.keep) row.keep(a.keep + r * a.D, on, kn);
   };
   if (base < a.rows) ask();
   for (; base < a.rows; base += stride) {
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
         w[e] = kept[e] ? w[e] * a.keep_scale : 0.f;
         dw[e] = kept[e] ? dw[e] * a.keep_scale : 0.f;
       }
-      if (post) v[e] = row.inside(e) ? (v[e] - st.x) * st.y : 0.f;          // normalised
+      if (post) v[e] = (v[e] - st.x) * st.y;          // normalised (behind the row's end it meets a gradient of zero)
     }
     if (pre) {
       float g[EPL], hat[EPL], s1 = 0.f, s2 = 0.f;
@@ -316,10 +320,11 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
       for (int e = 0; e < EPL; ++e) {
         const float vv = post ? fmaf(v[e], pg[e], pb[e]) : v[e];
         const float y = kept[e] ? fmaf(vv * w[e], sc[e], x[e]) : x[e];
-        hat[e] = row.inside(e) ? (y - st.z) * st.w : 0.f;
+        hat[e] = (y - st.z) * st.w;
         g[e] = d[e] * ng[e];
-        s1 += g[e];
-        s2 = fmaf(g[e], hat[e], s2);
+        const float gc = row.counted(e, g[e]);
+        s1 += gc;
+        s2 = fmaf(gc, hat[e], s2);
         sums[GATED_SUM_PRE_G][e] = fmaf(d[e], hat[e], sums[GATED_SUM_PRE_G][e]);
         sums[GATED_SUM_PRE_B][e] += d[e];
       }
@@ -341,14 +346,15 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
         sums[GATED_SUM_POST_B][e] += dv[e];
       }
     }
-    if (a.dz) row.store(row.at(reinterpret_cast<T*>(a.dz), mine, a.D), on, dw);
+    if (a.dz) row.store(reinterpret_cast<T*>(a.dz) + mine * a.D, on, dw);
     if (post) {
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
-        dv[e] = row.inside(e) ? dv[e] * pg[e] : 0.f;
-        s1 += dv[e];
-        s2 = fmaf(dv[e], v[e], s2);
+        dv[e] *= pg[e];
+        const float gc = row.counted(e, dv[e]);
+        s1 += gc;
+        s2 = fmaf(gc, v[e], s2);
       }
       const float2 m = team.sum(s1, s2);
       const float m1 = m.x * mean_weight, m2 = m.y * inv_D;
@@ -356,12 +362,12 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
       for (int e = 0; e < EPL; ++e) dv[e] = st.y * (dv[e] - fmaf(v[e], m2, m1));
     }
     if (a.u) {
-      if (a.du) row.store(row.at(reinterpret_cast<T*>(a.du), mine, a.D), on, dv);
+      if (a.du) row.store(reinterpret_cast<T*>(a.du) + mine * a.D, on, dv);
     } else {
 #pragma unroll
       for (int e = 0; e < EPL; ++e) t[e] += dv[e];
     }
-    if (a.dx) row.store(row.at(reinterpret_cast<T*>(a.dx), mine, a.D), on, t);
+    if (a.dx) row.store(reinterpret_cast<T*>(a.dx) + mine * a.D, on, t);
   }
   // column sums of the block: its teams in order
   float* part = a.part + (int64_t)blockIdx.x * GATED_SUMS * a.D;
@@ -388,22 +394,25 @@ __global__ __launch_bounds__(THREADS) void gated_norm_bwd_kernel(GatedNormArgs a
     if (TEAMS == 1 || threadIdx.x < TPR)
 #pragma unroll
       for (int e = 0; e < EPL; ++e)
-        if (row.inside(e)) part[(int64_t)s * a.D + row.col(e / R::N) + e % R::N] = sums[s][e];
+        if (row.own(e)) part[(int64_t)s * a.D + row.col(e)] = sums[s][e];
   }
 }
 
-// f(threads a row within a wave or 0, elements, the block's most threads, aligned), all constants.
+// f(threads a row within a wave or 0, elements, the block's most threads, kind of row), all constants.
 template <typename T, typename F>
 void for_shape(int dtype, int D, F f) {
   constexpr int N = MbvaeVec<T>::N;
   const GatedNormShape s = gated_norm_shape(dtype, D);
-  const auto with = [&](auto lanes, auto elements, auto threads) {
-    if (D % N == 0) f(lanes, elements, threads, std::true_type());
-    else f(lanes, elements, threads, std::false_type());
-  };
-#define GN_CASE(lanes, elements, threads) \
-  with(std::integral_constant<int, lanes>(), std::integral_constant<int, elements>(), std::integral_constant<int, threads>())
-  if (s.threads_a_row == 16) GN_CASE(16, N, 256);
+#define GN_INT(i) std::integral_constant<int, i>()
+#define GN_CASE(lanes, elements, threads)                                                              \
+  do {                                                                                                 \
+    if (D % N == 0) f(GN_INT(lanes), GN_INT(elements), GN_INT(threads), GN_INT(WHOLE));                \
+    else f(GN_INT(lanes), GN_INT(elements), GN_INT(threads), GN_INT(MOVED));                           \
+  } while (0)
+  if (D < N) f(GN_INT(4), GN_INT(N), GN_INT(256), GN_INT(SHORT));
+  else if (s.threads_a_row == 4) GN_CASE(4, N, 256);
+  else if (s.threads_a_row == 8) GN_CASE(8, N, 256);
+  else if (s.threads_a_row == 16) GN_CASE(16, N, 256);
   else if (s.threads_a_row == 32) GN_CASE(32, N, 256);
   else if (s.threads_a_row == 64 && s.elements == N) GN_CASE(64, N, 256);
   else if (s.threads_a_row == 64) GN_CASE(64, 8, 256);
@@ -411,16 +420,16 @@ void for_shape(int dtype, int D, F f) {
   else if (s.block <= 512) GN_CASE(0, 8, 512);
   else GN_CASE(0, 8, 1024);
 #undef GN_CASE
+#undef GN_INT
 }
 
 template <typename T>
 void gated_norm_launch(int dtype, bool forward, const GatedNormArgs& a, unsigned blocks, hipStream_t stream) {
   const unsigned threads = (unsigned)gated_norm_shape(dtype, a.D).block;
-  for_shape<T>(dtype, a.D, [&](auto lanes, auto elements, auto most, auto aligned) {
-    constexpr int TPR = decltype(lanes)::value, EPL = decltype(elements)::value, MOST = decltype(most)::value;
-    constexpr bool ALIGNED = decltype(aligned)::value;
-    if (forward) hipLaunchKernelGGL((gated_norm_fwd_kernel<T, TPR, EPL, MOST, ALIGNED>), dim3(blocks), dim3(threads), 0, stream, a);
-    else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, TPR, EPL, MOST, ALIGNED>), dim3(blocks), dim3(threads), 0, stream, a);
+  for_shape<T>(dtype, a.D, [&](auto lanes, auto elements, auto most, auto kind) {
+    constexpr int TPR = decltype(lanes)::value, EPL = decltype(elements)::value, MOST = decltype(most)::value, KIND = decltype(kind)::value;
+    if (forward) hipLaunchKernelGGL((gated_norm_fwd_kernel<T, TPR, EPL, MOST, KIND>), dim3(blocks), dim3(threads), 0, stream, a);
+    else hipLaunchKernelGGL((gated_norm_bwd_kernel<T, TPR, EPL, MOST, KIND>), dim3(blocks), dim3(threads), 0, stream, a);
   });
 }
 
