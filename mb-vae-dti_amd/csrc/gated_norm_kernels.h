@@ -5,6 +5,12 @@
 
 namespace {
 
+// 1 / a to within a rounding: the hardware's reciprocal and one Newton step.
+__device__ __forceinline__ float reciprocal(float a) {
+  const float r = __builtin_amdgcn_rcpf(a);
+  return fmaf(fmaf(-a, r, 1.f), r, r);
+}
+
 // ------------------------------------------------------------------------------------------------ sums over a row
 // TPR lanes of a wave own a row (4 to 64), or, with TPR == 0, a whole block does: its waves meet in LDS, in buffers that alternate so
 // that one barrier a sum is enough.
@@ -31,13 +37,46 @@ struct Team {
     if constexpr (TPR > 0) return mbvae_team_sum<TPR>(a);
     else return sum(a, 0.f).x;
   }
+  // Mean of the D values that the team's threads hold (t, where own) and the sum of their squared deviations from it, each summed from
+  // the values themselves.  A block needs one barrier for both: its waves exchange their own mean and deviations, count[w] values each.
+  template <int EPL, typename R>
+  __device__ __forceinline__ void moments(const R& row, const float* t, float inv_D, const float* count, float& mean, float& squares) {
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) s += row.counted(e, t[e]);
+    const auto deviations = [&](float m) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const float d = row.own(e) ? t[e] - m : 0.f;
+        q = fmaf(d, d, q);
+      }
+    };
+    if constexpr (TPR > 0) {
+      mean = sum(s) * inv_D;
+      deviations(mean);
+      squares = sum(q);
+    } else {
+      const unsigned wave = threadIdx.x >> 6, waves = blockDim.x / 64;
+      const float m = mbvae_team_sum<64>(s) * reciprocal(count[wave]);
+      deviations(m);
+      q = mbvae_team_sum<64>(q);
+      float2* r = red + turn * 16;
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0) r[wave] = make_float2(m, q);
+      __syncthreads();
+      float total = 0.f, within = 0.f, between = 0.f;
+      for (unsigned w = 0; w < waves; ++w) total = fmaf(count[w], r[w].x, total);
+      mean = total * inv_D;
+      for (unsigned w = 0; w < waves; ++w) {
+        const float d = r[w].x - mean;
+        within += r[w].y;
+        between = fmaf(count[w] * d, d, between);
+      }
+      squares = within + between;
+    }
+  }
 };
 
-// 1 / a to within a rounding: the hardware's reciprocal and one Newton step.
-__device__ __forceinline__ float reciprocal(float a) {
-  const float r = __builtin_amdgcn_rcpf(a);
-  return fmaf(fmaf(-a, r, 1.f), r, r);
-}
 // sigmoid(z) and its derivative, accurate at both ends: with t = exp(-|z|) they are 1 / (1 + t) or t / (1 + t), and t / (1 + t)^2.
 // t = 2^-(h + l) where h + l is |z| log2(e) to 48 bits: the hardware's 2^h, corrected by l to first order.
 __device__ __forceinline__ void sigmoid(float z, float& s, float& ds) {
@@ -144,24 +183,25 @@ struct Row {
   }
 };
 
-// Mean and reciprocal deviation of a row (two-pass: the deviations are summed from the mean).
+// Mean and reciprocal deviation of a row.
 template <int EPL, typename R, typename TeamT>
-__device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float* t, float inv_D, bool rms, float eps, float& mean, float& r) {
+__device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float* t, float inv_D, bool rms, float eps, const float* count, float& mean,
+                                          float& r) {
+  float squares;
   mean = 0.f;
-  if (!rms) {
-    float s = 0.f;
+  if (rms) {
+    float q = 0.f;
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) s += row.counted(e, t[e]);
-    mean = team.sum(s) * inv_D;
+    for (int e = 0; e < EPL; ++e) {
+      const float d = row.counted(e, t[e]);
+      q = fmaf(d, d, q);
+    }
+    squares = team.sum(q);
+  } else {
+    team.template moments<EPL>(row, t, inv_D, count, mean, squares);
   }
-  float q = 0.f;
-#pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    const float d = row.own(e) ? t[e] - mean : 0.f;
-    q = fmaf(d, d, q);
-  }
-  // 1 / sqrt(a) to within a rounding: the hardware's and one Newton step (none where that is not finite: eps = 0 and a row of zeros)
-  const float a = fmaf(team.sum(q), inv_D, eps), r0 = __builtin_amdgcn_rsqf(a), step = fmaf(r0 * -a, r0, 1.f);
+  // 1 / sqrt(a) to within a rounding: the hardware's and one Newton step (not where that leaves the range: eps = 0 and a row of zeros)
+  const float a = fmaf(squares, inv_D, eps), r0 = __builtin_amdgcn_rsqf(a), step = fmaf(r0 * -a, r0, 1.f);
   r = a > 1e-37f ? fmaf(0.5f * r0, step, r0) : 1.f / sqrtf(a);
 }
 
@@ -174,6 +214,15 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
   __shared__ float2 red[32];
   Team<TPR> team{red, 0};
   const R row(a.D);
+  __shared__ float count[16];                                       // a block's row: how many of its values each wave holds
+  if constexpr (TPR == 0) {
+    float mine = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) mine += row.own(e) ? 1.f : 0.f;
+    mine = mbvae_team_sum<64>(mine);
+    if ((threadIdx.x & 63) == 0) count[threadIdx.x >> 6] = mine;
+    __syncthreads();
+  }
   const float inv_D = 1.f / a.D;
   float pg[EPL], pb[EPL], ng[EPL], nb[EPL], sc[EPL];
   row.param(a.post_g, a.ptype, 0.f, pg);
@@ -222,7 +271,7 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
     if (base + stride < a.rows) ask();
     float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
     if (a.post_g) {
-      row_stats<EPL>(row, team, v, inv_D, a.rms, a.eps, st.x, st.y);
+      row_stats<EPL>(row, team, v, inv_D, a.rms, a.eps, count, st.x, st.y);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) v[e] = fmaf((v[e] - st.x) * st.y, pg[e], pb[e]);
     }
@@ -237,7 +286,7 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
     row.store(py, on, y);
     py += stride * a.D;
     if (a.pre_g) {
-      row_stats<EPL>(row, team, y, inv_D, a.rms, a.eps, st.z, st.w);
+      row_stats<EPL>(row, team, y, inv_D, a.rms, a.eps, count, st.z, st.w);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) y[e] = fmaf((y[e] - st.z) * st.w, ng[e], nb[e]);
       row.store(pn, on, y);
