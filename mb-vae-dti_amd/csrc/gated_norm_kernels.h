@@ -38,9 +38,9 @@ struct Team {
     else return sum(a, 0.f).x;
   }
   // Mean of the D values that the team's threads hold (t, where own) and the sum of their squared deviations from it, each summed from
-  // the values themselves.  A block needs one barrier for both: its waves exchange their own mean and deviations, count[w] values each.
+  // the values themselves.  A block needs one barrier for both: its waves exchange the mean and the deviations of what each holds.
   template <int EPL, typename R>
-  __device__ __forceinline__ void moments(const R& row, const float* t, float inv_D, const float* count, float& mean, float& squares) {
+  __device__ __forceinline__ void moments(const R& row, const float* t, float inv_D, float& mean, float& squares) {
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) s += row.counted(e, t[e]);
@@ -57,7 +57,7 @@ struct Team {
       squares = sum(q);
     } else {
       const unsigned wave = threadIdx.x >> 6, waves = blockDim.x / 64;
-      const float m = mbvae_team_sum<64>(s) * reciprocal(count[wave]);
+      const float m = mbvae_team_sum<64>(s) * reciprocal(row.held(wave));
       deviations(m);
       q = mbvae_team_sum<64>(q);
       float2* r = red + turn * 16;
@@ -65,12 +65,12 @@ struct Team {
       if ((threadIdx.x & 63) == 0) r[wave] = make_float2(m, q);
       __syncthreads();
       float total = 0.f, within = 0.f, between = 0.f;
-      for (unsigned w = 0; w < waves; ++w) total = fmaf(count[w], r[w].x, total);
+      for (unsigned w = 0; w < waves; ++w) total = fmaf(row.held(w), r[w].x, total);
       mean = total * inv_D;
       for (unsigned w = 0; w < waves; ++w) {
         const float d = r[w].x - mean;
         within += r[w].y;
-        between = fmaf(count[w] * d, d, between);
+        between = fmaf(row.held(w) * d, d, between);
       }
       squares = within + between;
     }
@@ -114,6 +114,14 @@ struct Row {
   // whether element e is one of the row's, and this thread's to count
   __device__ __forceinline__ bool own(int e) const { return there[e / N] && (ALIGNED || (col(e) >= first[e / N] && col(e) < D)); }
   __device__ __forceinline__ float counted(int e, float t) const { return ALIGNED || own(e) ? t : 0.f; }
+
+  // how many of the row's values wave w of a block holds
+  __device__ __forceinline__ float held(int w) const {
+    int n = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) n += min(max(D - (v * (int)blockDim.x + 64 * w) * N, 0), 64 * N);
+    return (float)n;
+  }
 
   // p: the row.  `on`: whether the row is there at all (a team behind the last row has zeros for all it loads)
   __device__ __forceinline__ void load(const T* p, bool on, Piece* out) const {
@@ -185,8 +193,7 @@ struct Row {
 
 // Mean and reciprocal deviation of a row.
 template <int EPL, typename R, typename TeamT>
-__device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float* t, float inv_D, bool rms, float eps, const float* count, float& mean,
-                                          float& r) {
+__device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float* t, float inv_D, bool rms, float eps, float& mean, float& r) {
   float squares;
   mean = 0.f;
   if (rms) {
@@ -198,7 +205,7 @@ __device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float
     }
     squares = team.sum(q);
   } else {
-    team.template moments<EPL>(row, t, inv_D, count, mean, squares);
+    team.template moments<EPL>(row, t, inv_D, mean, squares);
   }
   // 1 / sqrt(a) to within a rounding: the hardware's and one Newton step (not where that leaves the range: eps = 0 and a row of zeros)
   const float a = fmaf(squares, inv_D, eps), r0 = __builtin_amdgcn_rsqf(a), step = fmaf(r0 * -a, r0, 1.f);
@@ -207,22 +214,15 @@ __device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float
 
 // Both kernels walk over the rows with a fixed grid and ask for the next row's operands before the current row's results are stored: a
 // load behind a store would wait for it (one counter, in order).
+// Blocks of 16-bit rows are held to 128 registers, which lets 16 waves share a compute unit: their rows are short next to the exchanges
+// that a block waits for.  (fp32 would spill: 1024 values 133 -> 213 us.)
 template <typename T, int TPR, int EPL, int THREADS, int KIND>
-__global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a) {
+__global__ __launch_bounds__(THREADS, TPR == 0 && sizeof(T) == 2 ? 4 : 1) void gated_norm_fwd_kernel(GatedNormArgs a) {
   typedef Row<T, TPR, EPL, KIND> R;
   constexpr int TEAMS = TPR ? THREADS / (TPR ? TPR : 1) : 1, NV = R::NV;
   __shared__ float2 red[32];
   Team<TPR> team{red, 0};
   const R row(a.D);
-  __shared__ float count[16];                                       // a block's row: how many of its values each wave holds
-  if constexpr (TPR == 0) {
-    float mine = 0.f;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) mine += row.own(e) ? 1.f : 0.f;
-    mine = mbvae_team_sum<64>(mine);
-    if ((threadIdx.x & 63) == 0) count[threadIdx.x >> 6] = mine;
-    __syncthreads();
-  }
   const float inv_D = 1.f / a.D;
   float pg[EPL], pb[EPL], ng[EPL], nb[EPL], sc[EPL];
   row.param(a.post_g, a.ptype, 0.f, pg);
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
     if (base + stride < a.rows) ask();
     float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
     if (a.post_g) {
-      row_stats<EPL>(row, team, v, inv_D, a.rms, a.eps, count, st.x, st.y);
+      row_stats<EPL>(row, team, v, inv_D, a.rms, a.eps, st.x, st.y);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) v[e] = fmaf((v[e] - st.x) * st.y, pg[e], pb[e]);
     }
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(THREADS) void gated_norm_fwd_kernel(GatedNormArgs a
     row.store(py, on, y);
     py += stride * a.D;
     if (a.pre_g) {
-      row_stats<EPL>(row, team, y, inv_D, a.rms, a.eps, count, st.z, st.w);
+      row_stats<EPL>(row, team, y, inv_D, a.rms, a.eps, st.z, st.w);
 #pragma unroll
       for (int e = 0; e < EPL; ++e) y[e] = fmaf((y[e] - st.z) * st.w, ng[e], nb[e]);
       row.store(pn, on, y);
