@@ -121,6 +121,8 @@ struct Rows {
 // A backward of these nodes cannot be differentiated again: its results say so when that is tried.
 variable_list differentiable_once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& t : grads)                                    // (what the kernels wrote has no history of its own to hang the error on)
+    if (t.defined()) t = t.detach().requires_grad_(true);
   auto refuse = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " cannot be differentiated twice", grads.size());
   return (*refuse)(std::move(grads));
 }
@@ -327,15 +329,13 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
     TORCH_CHECK_VALUE(g.is_contiguous() || g.is_non_overlapping_and_dense(), what, ": a gradient must fill its memory densely, got strides ", g.strides(),
                       " for shape ", g.sizes());
     numel[i] = g.numel();
-    src[i] = g.const_data_ptr();
+    src[i] = write && !apart ? dst[i] = g.mutable_data_ptr() : g.const_data_ptr();
     if (apart) {
       const Tensor& o = out[i];
       TORCH_CHECK_VALUE(o.scalar_type() == g.scalar_type() && o.device() == device && o.sizes() == g.sizes() &&
                             (numel[i] <= 1 || o.strides() == g.strides()) && o.layout() == at::kStrided && !o.requires_grad(),
                         what, ": an output must have its gradient's type, shape, strides and device");
       dst[i] = o.mutable_data_ptr();
-    } else if (write) {
-      dst[i] = g.mutable_data_ptr();
     }
   }
   if (write)                                                 // (refused for tensors that may not be written here, so before the launch)

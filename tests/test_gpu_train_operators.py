@@ -426,6 +426,22 @@ def test_gated_residual_norm_gradient_against_differences(ops):
     assert abs((values[0] - values[1]) / (2 * step) - slope) <= 1e-3 * size
 
 
+def test_gated_residual_norm_cannot_be_differentiated_twice(ops):
+    g = _gen(14)
+    host = _block(g, (5, 24), F32, F32, True, True, False, True, True, True, "layer")
+    dev = {k: _device(v) if k not in ("keep_scale", "norm") else v for k, v in host.items()}
+    leaves = _leaves(dev)
+    y, n = _call(ops, dev, 1e-5)
+    once = torch.autograd.grad((y * n).sum(), list(leaves.values()), retain_graph=True)
+    graph = torch.autograd.grad((y * n).sum(), list(leaves.values()), create_graph=True)
+    for a, b in zip(once, graph):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="twice"):
+        graph[0].sum().backward(retain_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(graph[0].sum(), leaves["x"])
+
+
 def test_gated_residual_norm_refusals(ops):
     x = torch.zeros(4, 16, device="cuda")
     ones = torch.ones(16, device="cuda")
