@@ -862,3 +862,76 @@ def test_lightning_gradient_clipping_hook(ops):
     assert all(float(p.grad.abs().max()) <= 2.0 for p in model.lin.parameters())
     with pytest.raises(ValueError, match="gradient_clip_algorithm"):
         model.configure_gradient_clipping(opt, 1.0, "other")
+
+
+# ------------------------------------------------------------------------------------------------ past 32 bits
+FAR = (1 << 22) + 3                  # rows of 1024 values: the last ones lie behind 2^32 values and 2^33 bytes
+
+
+def _far_rows(seed):
+    """[FAR, 1024] bf16, every row its own: a row of noise scaled by a value that differs from its neighbours'."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    row = torch.randn(1024, generator=g, device="cuda").bfloat16()
+    factor = (torch.rand(FAR, 1, generator=g, device="cuda") + 0.5).bfloat16()
+    return row * factor
+
+
+LOOK = [0, 1, FAR // 2, (1 << 21) - 1, 1 << 21, (1 << 22) - 1, 1 << 22, FAR - 2, FAR - 1]
+
+
+def test_embedding_past_32_bits(ops):
+    table = _far_rows(1)
+    ids = torch.tensor([0, FAR - 1, 1 << 22, FAR - 1, 7, (1 << 21) + 5, FAR, -1], device="cuda")
+    got = ops.embedding(ids, table, 2.0)
+    want, bound = embedding_reference(torch.arange(6), torch.stack([table[i] for i in ids[:6].tolist()]), 2.0)
+    check(got[:6], want, bound, "far rows of the table")
+    assert not bool(got[6:].any())
+    weight = table.requires_grad_(True)
+    dy = torch.randn(8, 1024, device="cuda").bfloat16()
+    dw, = torch.autograd.grad(ops.embedding(ids, weight), weight, dy)
+    want, bound = embedding_gradient(torch.tensor([0, 1, 2, 1, 3, 4]), dy[:6], 5, 1.0)
+    check(dw[torch.tensor([0, FAR - 1, 1 << 22, 7, (1 << 21) + 5], device="cuda")], want, bound, "far rows of its gradient")
+    assert int(dw.any(1).sum()) == 5
+    del table, weight, dw
+    # as many tokens: few classes, then enough of them for the sort
+    dy = _far_rows(2)
+    for classes in (3, 40):
+        ids = (torch.arange(FAR, device="cuda") % (classes + 1)).to(torch.int8)          # (one id in classes + 1 is outside the table)
+        w = torch.randn(classes, 1024, device="cuda").bfloat16().requires_grad_(True)
+        y = ops.embedding(ids, w)
+        for r in LOOK:
+            k = r % (classes + 1)
+            assert torch.equal(y[r], w.detach()[k] if k < classes else torch.zeros_like(y[r]))
+        dw, = torch.autograd.grad(y, w, dy)
+        for k in (0, classes - 1):
+            mine = dy[k::classes + 1]
+            total = sum(mine[i:i + (1 << 18)].double().sum(0) for i in range(0, mine.shape[0], 1 << 18))
+            size = sum(mine[i:i + (1 << 18)].double().abs().sum(0) for i in range(0, mine.shape[0], 1 << 18))
+            check(dw[k], total, total.abs() * half_step(BF16) + size * U * 4096, "a class's gradient")      # (sums of at most 1024 by 4096 terms)
+        del y, dw
+
+
+def test_gated_residual_norm_past_32_bits(ops):
+    x, z = _far_rows(3), _far_rows(4)
+    gamma, beta = torch.ones(1024, device="cuda"), torch.zeros(1024, device="cuda")
+    dy = _far_rows(5)
+    leaves = [x.requires_grad_(True), z.requires_grad_(True)]
+    y, n = ops.gated_residual_norm(x, None, z, pre=(gamma, beta))
+    dx, dz = torch.autograd.grad([y, n], leaves, [dy, dy])
+    pick = torch.tensor(LOOK, device="cuda")
+    few = dict(x=x.detach()[pick], u=None, z=z.detach()[pick], keep=None, keep_scale=1.0, post=None, scale=None, pre=(gamma, beta), norm="layer")
+    want = gated_reference(**few, eps=1e-5, dy=dy[pick], dn=dy[pick])
+    for k, t in (("y", y), ("n", n), ("dx", dx), ("dz", dz)):
+        check(t[pick], *want[k], k)
+
+
+def test_clip_grad_norm_past_32_bits(ops):
+    big = _far_rows(6)
+    small = torch.ones(3, device="cuda")
+    norm = ops.global_grad_norm([small, big])
+    total = sum(big[i:i + (1 << 18)].double().square().sum() for i in range(0, FAR, 1 << 18)) + 3
+    check(norm, total.sqrt(), float(total.sqrt()) * 2 * U, "norm")
+    pick = torch.tensor(LOOK, device="cuda")
+    before = big[pick].double()
+    ops.clip_grad_norm_([small, big], 0.25 * float(norm))
+    check(big[pick], before * 0.25, before.abs() * (half_step(BF16) + 8 * U), "clipped")
