@@ -70,18 +70,16 @@ __device__ __forceinline__ int tensor_of(const Table& t, uint32_t c) {
 }
 __device__ __forceinline__ uint32_t share_begin(uint32_t chunks, uint32_t block, uint32_t blocks) { return (uint32_t)((uint64_t)chunks * block / blocks); }
 
-// f(tensor, its first value here, values here) for the tensors of chunks [c0, c1), from the last to the first.
-template <typename Table, typename F>
-__device__ __forceinline__ void walk_back(const Table& t, uint32_t c0, uint32_t c1, F f) {
+// f(tensor, its first value here, values here) for the tensors of the chunks [c0, c1), from the first to the last or the other way.
+template <bool BACK, typename Table, typename F>
+__device__ __forceinline__ void walk(const Table& t, uint32_t c0, uint32_t c1, F f) {
   if (c0 >= c1) return;
-  int i = tensor_of(t, c1 - 1);
-  while (c1 > c0) {
-    const uint32_t first = t.first(i), from = max(c0, first);
-    const bool whole = c1 == t.first(i + 1);                       // (else the share ends inside the tensor)
-    const int64_t n = (int64_t)(c1 - from - 1) * CHUNK + (whole ? t.last(i) & 0xffffff : CHUNK);
+  for (int i = tensor_of(t, BACK ? c1 - 1 : c0); c0 < c1; i += BACK ? -1 : 1) {
+    const uint32_t first = t.first(i), behind = t.first(i + 1), from = max(c0, first), to = min(c1, behind);
+    const int64_t n = (int64_t)(to - from - 1) * CHUNK + (to == behind ? t.last(i) & 0xffffff : CHUNK);      // (else the share ends inside the tensor)
     f(i, (int64_t)(from - first) * CHUNK, n);
-    c1 = from;
-    --i;
+    if (BACK) c1 = from;
+    else c0 = to;
   }
 }
 
@@ -152,7 +150,7 @@ template <int P, typename Table>
 __global__ __launch_bounds__(THREADS) void grad_norm_kernel(Table t, uint32_t chunks, double* __restrict__ part) {
   double acc[4] = {0., 0., 0., 0.};
   uint32_t top = 0;
-  walk_back(t, share_begin(chunks, blockIdx.x, gridDim.x), share_begin(chunks, blockIdx.x + 1, gridDim.x), [&](int i, int64_t at, int64_t n) {
+  walk<false>(t, share_begin(chunks, blockIdx.x, gridDim.x), share_begin(chunks, blockIdx.x + 1, gridDim.x), [&](int i, int64_t at, int64_t n) {
     const int dtype = t.last(i) >> 24;
     if (dtype == MBVAE_F32) norm_span<P>(reinterpret_cast<const float*>(t.src(i)) + at, n, acc, top);
     else if (dtype == MBVAE_BF16) norm_span<P>(reinterpret_cast<const mbvae_bf16*>(t.src(i)) + at, n, acc, top);
@@ -223,7 +221,7 @@ __global__ __launch_bounds__(THREADS) void grad_scale_kernel(Table t, uint32_t c
   const double c = max_norm / (a + 1e-6);
   const float f = c > 1. || max_norm == INFINITY ? 1.f : (float)c;        // (a NaN norm makes every gradient NaN)
   if (in_place && f == 1.f) return;                        // nothing to scale: the values stay as they are
-  walk_back(t, share_begin(chunks, blockIdx.x, gridDim.x), share_begin(chunks, blockIdx.x + 1, gridDim.x), [&](int i, int64_t at, int64_t n) {
+  walk<true>(t, share_begin(chunks, blockIdx.x, gridDim.x), share_begin(chunks, blockIdx.x + 1, gridDim.x), [&](int i, int64_t at, int64_t n) {
     const int dtype = t.last(i) >> 24;
     if (dtype == MBVAE_F32) scale_span(reinterpret_cast<const float*>(t.src(i)) + at, reinterpret_cast<float*>(t.dst(i)) + at, n, f);
     else if (dtype == MBVAE_BF16) scale_span(reinterpret_cast<const mbvae_bf16*>(t.src(i)) + at, reinterpret_cast<mbvae_bf16*>(t.dst(i)) + at, n, f);
