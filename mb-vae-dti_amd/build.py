@@ -18,7 +18,8 @@ SOURCES = ["gemm.hip", "edge_attn.hip", "edge_fused.hip", "rowops.hip", "loss.hi
 # source is bit-stable next to them (tools/concurrency_probe.py, tests/test_gpu_concurrency.py).  The train step's time is
 # the same with and without (54.5-54.9 ms either way): the row kernels are memory bound and the matrix kernels' epilogues
 # do not depend on packed issue.  The host pass does not know the feature and says so; that warning is filtered below.
-FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-ffp-contract=on",
+# A 64-bit count that becomes a 32-bit one without a cast is an error: tensors pass 2^31 values here.
+FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-ffp-contract=on", "-Werror=shorten-64-to-32",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 

@@ -196,7 +196,8 @@ template <typename T>
 __device__ __forceinline__ void fill_zero(T* p, int64_t values, int64_t block, int64_t blocks) {
   constexpr int N = MbvaeVec<T>::N;
   const float zero[N] = {};
-  for (int64_t i = (block * blockDim.x + threadIdx.x) * N; i < values; i += blocks * blockDim.x * N) mbvae_store_vec<T>(p + i, values - i, zero);
+  for (int64_t i = (block * blockDim.x + threadIdx.x) * N; i < values; i += blocks * blockDim.x * N)
+    mbvae_store_vec<T>(p + i, (int)min(values - i, (int64_t)N), zero);         // (what is left of a table may not fit 32 bits)
 }
 __device__ __forceinline__ void fill_zero_any(void* p, int dtype, int64_t values, int64_t block, int64_t blocks) {
   if (dtype == MBVAE_F32) fill_zero(reinterpret_cast<float*>(p), values, block, blocks);

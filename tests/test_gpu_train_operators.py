@@ -935,3 +935,24 @@ def test_clip_grad_norm_past_32_bits(ops):
     before = big[pick].double()
     ops.clip_grad_norm_([small, big], 0.25 * float(norm))
     check(big[pick], before * 0.25, before.abs() * (half_step(BF16) + 8 * U), "clipped")
+
+
+@pytest.mark.parametrize("V,D", [((1 << 21) + 3, 1024), ((1 << 22) + 3, 1024), ((1 << 20) + 1, 3 * 1024 + 5), (131075, 16385)])
+@pytest.mark.parametrize("rows", [0, 7])
+def test_embedding_gradient_clears_tables_past_32_bits(ops, rows, V, D):
+    """Every row of the table's gradient that no token has is written, whatever lay in its place: tables just past 2^31 and 2^32 values and between
+    them, through the C entry into memory full of NaN, by the radix sort, by one ordering launch (the last table) and without any token."""
+    from mbvae_amd import _lib
+    ids = torch.tensor([0, V - 1, 1 << 16, V - 1, 5, V, -1], device="cuda")[:rows]
+    dy = torch.randn(rows, D, generator=_gen(D)).bfloat16().cuda()
+    dw = torch.full((V, D), math.nan, dtype=BF16, device="cuda")
+    ws = torch.empty(max(16, _lib.query("mbvae_embedding_bwd_workspace", rows, V, D, 1)), dtype=torch.uint8, device="cuda")
+    _lib.call("mbvae_embedding_bwd", ids.data_ptr(), 8, dy.data_ptr(), D, dw.data_ptr(), rows, V, D, 1.0, 1, ws.data_ptr(), ws.numel(),
+              torch.cuda.current_stream().cuda_stream)
+    if rows:
+        want, bound = embedding_gradient(torch.tensor([0, 1, 2, 1, 3]), dy[:5], 4, 1.0)
+        taken = torch.tensor([0, V - 1, 1 << 16, 5], device="cuda")
+        check(dw[taken], want, bound, "rows with tokens")
+        dw[taken] = 0
+    for r in range(0, V, 1 << 18):
+        assert not bool(dw[r:r + (1 << 18)].any()), f"rows {r} to {r + (1 << 18)} hold values that nobody has written"
