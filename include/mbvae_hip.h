@@ -147,7 +147,7 @@ int mbvae_gate_bwd(const float* dy, const float* u, const float* z, const uint8_
  * added, whatever v and z hold there.  scale, gammas, betas: [D] of type ptype; post_gamma == NULL / pre_gamma == NULL: that norm is
  * absent (n is then not written); a beta may be NULL.  rms: root-mean-square norms, no mean is taken out.  x, u, z, dy, dn: rows ld*
  * elements apart, elements of a row contiguous, any alignment; outputs contiguous, sharing no memory with inputs.  dtype / ptype: 0 fp32, 1 bf16, 2 fp16; all
- * arithmetic is fp32.  1 <= D <= 8192, rows < 2^31.  stats (float [rows, 4], 16-byte aligned): written by the forward for the
+ * arithmetic is fp32; a row whose sum of squares is beyond fp32 normalises to 0.  1 <= D <= 8192, rows < 2^31.  stats (float [rows, 4], 16-byte aligned): written by the forward for the
  * backward, NULL where there is none.
  * Backward: dy / dn NULL: that output has no gradient.  du only where u was given, dz only where z was; any output may be NULL; with
  * u == NULL dx is the whole gradient of x.  dscale ... dpre_beta: [D] of type ptype, overwritten.  workspace: at least

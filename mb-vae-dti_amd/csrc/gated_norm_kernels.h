@@ -207,9 +207,10 @@ __device__ __forceinline__ void row_stats(const R& row, TeamT& team, const float
   } else {
     team.template moments<EPL>(row, t, inv_D, mean, squares);
   }
-  // 1 / sqrt(a) to within a rounding: the hardware's and one Newton step (not where that leaves the range: eps = 0 and a row of zeros)
+  // 1 / sqrt(a) to within a rounding: the hardware's and one Newton step.  Not where that leaves the range: eps = 0 and a row of zeros; a sum of
+  // squares beyond fp32, which is infinite here - r is 0, and what is finite of such a row becomes 0 (and not NaN).
   const float a = fmaf(squares, inv_D, eps), r0 = __builtin_amdgcn_rsqf(a), step = fmaf(r0 * -a, r0, 1.f);
-  r = a > 1e-37f ? fmaf(0.5f * r0, step, r0) : 1.f / sqrtf(a);
+  r = a > 1e-37f && a < INFINITY ? fmaf(0.5f * r0, step, r0) : 1.f / sqrtf(a);
 }
 
 // Both kernels walk over the rows with a fixed grid and ask for the next row's operands before the current row's results are stored: a

@@ -386,7 +386,8 @@ def gated_residual_norm(x, u=None, z=None, keep=None, keep_scale=1.0, post=None,
     itself is gated.  z None: no gate.  keep: dropout mask (uint8 or bool, x's shape); where it is 0 nothing is added, whatever u and z
     hold.  post / pre: (gamma, beta) or (gamma, None) of the norm behind the block and of the one that opens the next; None: absent.
     res_scale: [D].  gamma, beta and res_scale share one type, float32 or any other of the three.  norm: "layer" or "rms".  Sums, statistics
-    and intermediate values are float32, outputs are rounded once (n comes from the unrounded y).  1 <= D <= 8192.  The gate and
+    and intermediate values are float32, outputs are rounded once (n comes from the unrounded y); a row whose sum of squares is beyond
+    float32 normalises to 0, as in ln_residual.  1 <= D <= 8192.  The gate and
     norm of mb_vae_dti/training/models/blocks.py:92-129, :318-328 (gate_update and ln_residual are the separate forms)."""
     if norm != "layer" and norm != "rms":
         raise ValueError(f"gated_residual_norm: norm is 'layer' or 'rms', got {norm!r}")

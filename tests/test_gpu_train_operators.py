@@ -956,3 +956,39 @@ def test_embedding_gradient_clears_tables_past_32_bits(ops, rows, V, D):
         dw[taken] = 0
     for r in range(0, V, 1 << 18):
         assert not bool(dw[r:r + (1 << 18)].any()), f"rows {r} to {r + (1 << 18)} hold values that nobody has written"
+
+
+@pytest.mark.parametrize("D,dtype", [(5, F32), (64, F32), (300, BF16), (512, F32), (520, BF16), (1037, F32), (4100, F32)])
+def test_gated_residual_norm_rows_whose_squares_leave_fp32(ops, D, dtype):
+    """A row of finite values whose mean square is beyond fp32 normalises to 0, as in the separate LayerNorm kernel (n is beta exactly, the
+    norm passes no gradient on); one infinity in a row takes only itself with it under the root mean square.  Other rows do not notice."""
+    g = _gen(D)
+    x, u = _randn(g, 9, D), _randn(g, 9, D)
+    x[3], x[7], u[4] = x[3] * 1e25, -3e24, u[4] * 1e25
+    x, u = x.to(dtype), u.to(dtype)
+    gamma, beta, dy, dn = 1 + 0.2 * _randn(g, D), _randn(g, D), _randn(g, 9, D, dtype=dtype), _randn(g, 9, D, dtype=dtype)
+    gamma, beta = gamma.cuda(), beta.cuda()
+    for norm in ("layer", "rms"):
+        leaves = [t.cuda().requires_grad_(True) for t in (x, u)]
+        y, n = ops.gated_residual_norm(*leaves, post=(gamma, beta), pre=(gamma, beta), norm=norm)
+        dx, du = torch.autograd.grad([y, n], leaves, [dy.cuda(), dn.cuda()])
+        assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(n).all()) and bool(torch.isfinite(dx).all()) and bool(torch.isfinite(du).all())
+        assert not bool(du[4].any()) and torch.equal(dx[3].cpu(), dy[3]), "a norm without scale passes no gradient on"
+        want = beta.to(dtype)
+        assert torch.equal(n[3], want) and torch.equal(y[4], (x[4].cuda().float() + beta).to(dtype))
+        if norm == "rms":                                  # (a row of equal values has no spread: LayerNorm sees a mean square within range)
+            assert torch.equal(n[7], want)
+        for i in (0, 1, 2, 5, 6, 8):
+            few = dict(x=x[i:i + 1], u=u[i:i + 1], z=None, keep=None, keep_scale=1.0, post=(gamma, beta), scale=None, pre=(gamma, beta), norm=norm)
+            ref = gated_reference(**few, eps=1e-5, dy=dy[i:i + 1], dn=dn[i:i + 1])
+            for k, t in (("y", y), ("n", n), ("dx", dx), ("du", du)):
+                check(t[i:i + 1], *ref[k], f"{k}, row {i}")
+    if dtype == F32:
+        plain = ops.ln_residual(x.cuda(), None, gamma, beta)
+        _, n = ops.gated_residual_norm(x.cuda(), torch.zeros_like(x).cuda(), pre=(gamma, beta))
+        assert torch.equal(torch.isnan(n), torch.isnan(plain)) and torch.equal(n[3], plain[3])
+    row = _randn(g, 2, D, dtype=dtype)
+    row[0, D // 2] = math.inf
+    _, n = ops.gated_residual_norm(row.cuda(), torch.zeros_like(row).cuda(), pre=(gamma, None), norm="rms")
+    rest = torch.arange(D, device="cuda") != D // 2
+    assert bool(torch.isnan(n[0, D // 2])) and not bool(n[0, rest].any()) and bool(torch.isfinite(n[1]).all())
