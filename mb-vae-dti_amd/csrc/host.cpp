@@ -94,10 +94,15 @@ Tensor part_of(const Tensor& flat, int64_t at, int64_t n) {
   return Tensor(std::move(impl));
 }
 
+// A tangent would be lost without a word: the kernels know nothing of it.
+void check_no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what, " has no forward-mode derivative (an operand carries a tangent)");
+}
 void check_typed(const Tensor& t, const char* what, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.layout() == at::kStrided && type_code(t.scalar_type()) >= 0, what, ": ", name,
               ": expected a dense float32, bfloat16 or float16 tensor on the GPU (got ", name_of(t.scalar_type()), " on ", t.device(),
               "); the HIP path has no CPU fallback");
+  check_no_tangent(t, what);
 }
 void check_same(const Tensor& t, const Tensor& as, const char* what, const char* name) {
   check_typed(t, what, name);
@@ -325,6 +330,7 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
     TORCH_CHECK(g.is_cuda() && g.device() == device, what, ": all gradients must be on one GPU; the HIP path has no CPU fallback");
     types[i] = type_code(g.scalar_type());
     TORCH_CHECK(types[i] >= 0 && g.layout() == at::kStrided, what, ": expected dense float32, bfloat16 or float16 gradients, got ", g.scalar_type());
+    check_no_tangent(g, what);
     TORCH_CHECK_VALUE(!g.requires_grad(), what, ": expected gradients (p.grad), got a tensor that requires gradients itself");
     TORCH_CHECK_VALUE(g.is_contiguous() || g.is_non_overlapping_and_dense(), what, ": a gradient must fill its memory densely, got strides ", g.strides(),
                       " for shape ", g.sizes());
@@ -335,6 +341,7 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
       TORCH_CHECK_VALUE(o.scalar_type() == g.scalar_type() && o.device() == device && o.sizes() == g.sizes() &&
                             (numel[i] <= 1 || o.strides() == g.strides()) && o.layout() == at::kStrided && !o.requires_grad(),
                         what, ": an output must have its gradient's type, shape, strides and device");
+      check_no_tangent(o, what);
       dst[i] = o.mutable_data_ptr();
     }
   }

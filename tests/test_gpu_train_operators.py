@@ -992,3 +992,35 @@ def test_gated_residual_norm_rows_whose_squares_leave_fp32(ops, D, dtype):
     _, n = ops.gated_residual_norm(row.cuda(), torch.zeros_like(row).cuda(), pre=(gamma, None), norm="rms")
     rest = torch.arange(D, device="cuda") != D // 2
     assert bool(torch.isnan(n[0, D // 2])) and not bool(n[0, rest].any()) and bool(torch.isfinite(n[1]).all())
+
+
+def test_forward_mode_is_refused(ops):
+    """An operand with a tangent: an error, not a result whose tangent is gone - whether or not anything also asks for a reverse pass."""
+    import torch.autograd.forward_ad as forward_ad
+    g = _gen(70)
+    ids = torch.tensor([0, 2, 1], device="cuda")
+    host = _block(g, (3, 8), F32, F32, True, True, False, True, True, True, "layer")
+    dev = {k: _device(v, False) if k not in ("keep_scale", "norm") else v for k, v in host.items()}
+    plain = torch.ones(3, 8, device="cuda")
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t.detach(), torch.ones_like(t))
+
+        for leaf in (False, True):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.embedding(ids, dual(plain.clone().requires_grad_(leaf)))
+            for k, b in ([(k, {**dev, k: dual(dev[k])}) for k in ("x", "u", "z", "scale")]
+                         + [(k, {**dev, k: pair}) for k in ("post", "pre") for pair in ((dual(dev[k][0]), dev[k][1]), (dev[k][0], dual(dev[k][1])))]):
+                b["z"] = b["z"].requires_grad_(leaf) if k != "z" else b["z"]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    _call(ops, b, 1e-5)
+                b["z"].requires_grad_(False)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.global_grad_norm([plain, dual(plain)])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.clip_grad_norm_([dual(plain.clone())], 1.0)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.clip_grad_norm_([plain], 1.0, out=[dual(plain.clone())])
+        assert ops.embedding(ids, plain).shape == (3, 8) and bool((plain == 1).all())
+    y, n = _call(ops, dev, 1e-5)
+    assert bool(torch.isfinite(n).all())
