@@ -178,16 +178,16 @@ __global__ __launch_bounds__(THREADS) void grad_norm_final_kernel(const double* 
   if (threadIdx.x == 0) *norm = (float)a;
 }
 
-// q = p * f over n values, the last ones first.
+// q = p * f * 2^e over n values, the last ones first.
 template <typename T>
-__device__ __forceinline__ void scale_span(const T* p, T* q, int64_t n, float f) {
+__device__ __forceinline__ void scale_span(const T* p, T* q, int64_t n, float f, int e2) {
   constexpr int N = MbvaeVec<T>::N, STEP = THREADS * N;
   typedef typename MbvaeVec<T>::Aligned V;
   typedef typename MbvaeVec<T>::Any A;
   const auto put = [&](T* to, const V& v, int left) {
     float w[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) w[e] = (float)v[e] * f;
+    for (int e = 0; e < N; ++e) w[e] = __builtin_amdgcn_ldexpf((float)v[e] * f, e2);
     mbvae_store_vec<T>(to, left, w);
   };
   int64_t at = n / (U * STEP) * (U * STEP);                          // what lies behind the last whole group comes first
@@ -219,13 +219,15 @@ __global__ __launch_bounds__(THREADS) void grad_scale_kernel(Table t, uint32_t c
   const double a = join_partials<P>(part, parts);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)a;
   const double c = max_norm / (a + 1e-6);
-  const float f = c > 1. || max_norm == INFINITY ? 1.f : (float)c;        // (a NaN norm makes every gradient NaN)
+  float f = c > 1. || max_norm == INFINITY ? 1.f : (float)c;              // (a NaN norm makes every gradient NaN)
+  int e = 0;
+  if (c > 0. && c < 1.17549435e-38) f = (float)frexp(c, &e);              // a factor below fp32's normal range would lose its bits
   if (in_place && f == 1.f) return;                        // nothing to scale: the values stay as they are
   walk<true>(t, share_begin(chunks, blockIdx.x, gridDim.x), share_begin(chunks, blockIdx.x + 1, gridDim.x), [&](int i, int64_t at, int64_t n) {
     const int dtype = t.last(i) >> 24;
-    if (dtype == MBVAE_F32) scale_span(reinterpret_cast<const float*>(t.src(i)) + at, reinterpret_cast<float*>(t.dst(i)) + at, n, f);
-    else if (dtype == MBVAE_BF16) scale_span(reinterpret_cast<const mbvae_bf16*>(t.src(i)) + at, reinterpret_cast<mbvae_bf16*>(t.dst(i)) + at, n, f);
-    else scale_span(reinterpret_cast<const mbvae_f16*>(t.src(i)) + at, reinterpret_cast<mbvae_f16*>(t.dst(i)) + at, n, f);
+    if (dtype == MBVAE_F32) scale_span(reinterpret_cast<const float*>(t.src(i)) + at, reinterpret_cast<float*>(t.dst(i)) + at, n, f, e);
+    else if (dtype == MBVAE_BF16) scale_span(reinterpret_cast<const mbvae_bf16*>(t.src(i)) + at, reinterpret_cast<mbvae_bf16*>(t.dst(i)) + at, n, f, e);
+    else scale_span(reinterpret_cast<const mbvae_f16*>(t.src(i)) + at, reinterpret_cast<mbvae_f16*>(t.dst(i)) + at, n, f, e);
   });
 }
 

@@ -1024,3 +1024,18 @@ def test_forward_mode_is_refused(ops):
         assert ops.embedding(ids, plain).shape == (3, 8) and bool((plain == 1).all())
     y, n = _call(ops, dev, 1e-5)
     assert bool(torch.isfinite(n).all())
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+@pytest.mark.parametrize("dtype,value,max_norm", [(F32, 3e38, 1e-3), (F32, -3e38, 1e-12), (BF16, 2e38, 1e-2), (F32, 3e38, 1.0), (F32, 1e-3, 1e-38), (F16, 6e4, 1e-35)])
+def test_clip_grad_norm_by_a_factor_below_fp32(ops, dtype, value, max_norm, p):
+    """A factor max_norm / norm below the smallest normal fp32 number keeps its bits: outputs to the same bound as any other."""
+    grads = [torch.full((1000,), value, dtype=dtype), torch.linspace(-1, 1, 777).to(dtype) * value, torch.zeros(5, dtype=dtype)]
+    _, _, want, bounds = clip_reference(grads, max_norm, p)
+    dev = [t.cuda() for t in grads]
+    out = [torch.full_like(t, 7.0) for t in dev]
+    ops.clip_grad_norm_(dev, max_norm, p, out=out)
+    ops.clip_grad_norm_(dev, max_norm, p)
+    for i, (o, d) in enumerate(zip(out, dev)):
+        check(o, want[i], bounds[i], f"output {i}")
+        assert torch.equal(o, d), "in place and into an output differ"
