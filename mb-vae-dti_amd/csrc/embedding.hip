@@ -37,7 +37,8 @@ __device__ __forceinline__ Id load_id(const void* ids, int type, int64_t r) {
 __device__ __forceinline__ uint32_t load_key(const void* ids, int type, int64_t r, uint32_t V) { return load_id(ids, type, r).key(V); }
 
 // ------------------------------------------------------------------------------------------------ forward
-// 2^LOG lanes own 16 bytes each of FWD_ROWS rows; a block's rows are neighbours and blockIdx.y counts its columns.  There is no loop: a
+// 2^LOG lanes own 16 bytes each of FWD_ROWS rows; a block's rows are neighbours, blockIdx.y counts its columns and blockIdx.z what grid x
+// cannot hold.  There is no loop: a
 // load behind a store waits for the store (one counter, in order), and a loop over rows spent more on addresses than on moving 16 bytes.
 // All ids are asked for before the first table row, and those before the first store.  The pairs of 256 graphs (1 M x 64 fp32):
 // 47.5 us = 5.7 TB/s of stores; with the rows in a grid-stride loop 65 us, with 1, 2 or 8 rows a thread 66, 53 and 48 us.
@@ -47,7 +48,7 @@ __device__ __forceinline__ void embedding_fwd_rows(const void* __restrict__ ids,
                                                    unsigned D, float scale, int log_lanes) {
   constexpr unsigned N = MbvaeVec<T>::N, U = FWD_ROWS;
   const unsigned teams = 256u >> log_lanes, team = threadIdx.x >> log_lanes, lane = threadIdx.x & ((1u << log_lanes) - 1);
-  const unsigned r0 = blockIdx.x * (teams * U) + team, col = ((blockIdx.y << log_lanes) + lane) * N;
+  const unsigned r0 = (blockIdx.z * gridDim.x + blockIdx.x) * (teams * U) + team, col = ((blockIdx.y << log_lanes) + lane) * N;
   if (r0 >= rows || col >= D) return;
   Id id[U];
   typename MbvaeVec<T>::Aligned t[U];
@@ -136,7 +137,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void embedding_few_join_kernel(const float* __restrict__ part, T* __restrict__ dW, int blocks, int64_t values, float scale) {
   __shared__ float red[32][9];
   const int cx = threadIdx.x & 7, g = threadIdx.x >> 3;
-  const int64_t c = (int64_t)blockIdx.x * 8 + cx;
+  const int64_t c = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 8 + cx;
   float a[8] = {};
   if (c < values) {
     int b = g;
@@ -537,6 +538,12 @@ int lanes_for(int64_t pieces, int most) {
   return l;
 }
 
+// Blocks of 256 threads over grid x and z: a grid has at most 2^32 - 1 threads along each of its sides.
+dim3 grid_of(int64_t blocks) {
+  const int64_t sheets = (blocks + (1 << 23) - 1) >> 23;
+  return dim3((unsigned)((blocks + sheets - 1) / sheets), 1, (unsigned)sheets);
+}
+
 // Tokens a chunk holds.  A chunk is one team's work: enough chunks to fill the chip, and at least 16 tokens so that the two rows of
 // partials a chunk may leave stay small next to what it reads.
 int chunk_for(int64_t rows, int64_t D) {
@@ -601,7 +608,8 @@ template <typename T>
 void launch_fwd(const void* ids, int id_type, const void* W, void* y, int64_t rows, int64_t V, int64_t D, float scale, hipStream_t stream) {
   const int lanes = lanes_for((D + vec<T>() - 1) / vec<T>(), 256), log_lanes = __builtin_ctz(lanes);
   const int64_t block_rows = FWD_ROWS * (256 / lanes), width = (int64_t)lanes * vec<T>();
-  const dim3 grid((unsigned)((rows + block_rows - 1) / block_rows), (unsigned)((D + width - 1) / width));
+  dim3 grid = grid_of((rows + block_rows - 1) / block_rows);
+  grid.y = (unsigned)((D + width - 1) / width);
   if (D % vec<T>() == 0)
     hipLaunchKernelGGL((embedding_fwd_kernel<T, true>), grid, dim3(256), 0, stream, ids, id_type, reinterpret_cast<const T*>(W), reinterpret_cast<T*>(y),
                        (unsigned)rows, (uint32_t)V, (unsigned)D, scale, log_lanes);
@@ -633,7 +641,7 @@ int launch_bwd(const Plan& p, const void* ids, int id_type, const T* dy, int64_t
     if (!MBVAE_ALLOW_BIG_LDS(embedding_few_kernel<T>)) return MBVAE_ELAUNCH;
     hipLaunchKernelGGL((embedding_few_kernel<T>), dim3((unsigned)p.blocks, (unsigned)((D + width - 1) / width)), dim3(256), V * vec<T>() * 1024, stream,
                        ids, id_type, dy, ldy, part, rows, (uint32_t)V, D, p.lanes);
-    hipLaunchKernelGGL((embedding_few_join_kernel<T>), dim3((unsigned)((values + 7) / 8)), dim3(256), 0, stream, part, dW, (int)p.blocks, values, scale);
+    hipLaunchKernelGGL((embedding_few_join_kernel<T>), grid_of((values + 7) / 8), dim3(256), 0, stream, part, dW, (int)p.blocks, values, scale);
     return mbvae_launch_status();
   }
   if (p.route == FEW_TOKENS) {

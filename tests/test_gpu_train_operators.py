@@ -1039,3 +1039,32 @@ def test_clip_grad_norm_by_a_factor_below_fp32(ops, dtype, value, max_norm, p):
     for i, (o, d) in enumerate(zip(out, dev)):
         check(o, want[i], bounds[i], f"output {i}")
         assert torch.equal(o, d), "in place and into an output differ"
+
+
+@pytest.mark.parametrize("V,dtype", [(16, F32), (16, BF16), (40, F16)])
+def test_embedding_of_the_widest_rows(ops, V, dtype):
+    """Rows of 2^23 values.  With 16 classes the join of the blocks' tables has 2^27 values, more than one side of a grid holds; 40 are ordered."""
+    D = 1 << 23
+    dy = torch.randn(3, D, device="cuda").to(dtype)
+    ids = torch.tensor([0, V - 1, V - 1], device="cuda")
+    weight = torch.randn(V, D, device="cuda").to(dtype).requires_grad_(True)
+    y = ops.embedding(ids, weight)
+    assert torch.equal(y, weight.detach()[ids])
+    dw, = torch.autograd.grad(y, weight, dy)
+    assert torch.equal(dw[0], dy[0]) and torch.equal(dw[V - 1], (dy[1].float() + dy[2].float()).to(dtype)) and not bool(dw[1:V - 1].any())
+
+
+def test_embedding_forward_past_one_side_of_a_grid(ops):
+    """2^26 rows of 516 values take 2^24 blocks of 256 threads: more than one side of a grid holds."""
+    rows, D = 1 << 26, 516
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < rows * D * 4 + (8 << 30):
+        pytest.skip("138 GB of output do not fit")
+    ids = (torch.arange(rows, device="cuda") % 7 - 1).to(torch.int8)
+    table = torch.randn(5, D, device="cuda")
+    padded = torch.cat((torch.zeros(1, D, device="cuda"), table, torch.zeros(1, D, device="cuda")))
+    y = ops.embedding(ids, table)
+    for r in range(0, rows, 1 << 20):
+        assert torch.equal(y[r:r + (1 << 20)], padded[ids[r:r + (1 << 20)].long() + 1]), f"rows from {r}"
+    del y
+    torch.cuda.empty_cache()
