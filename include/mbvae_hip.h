@@ -149,7 +149,8 @@ int mbvae_gate_bwd(const float* dy, const float* u, const float* z, const uint8_
  * elements apart, elements of a row contiguous, any alignment; outputs contiguous, sharing no memory with inputs.  dtype / ptype: 0 fp32, 1 bf16, 2 fp16; all
  * arithmetic is fp32; a row whose sum of squares is beyond fp32 normalises to 0.  1 <= D <= 8192, rows < 2^31.  stats (float [rows, 4], 16-byte aligned): written by the forward for the
  * backward, NULL where there is none.
- * Backward: dy / dn NULL: that output has no gradient.  du only where u was given, dz only where z was; any output may be NULL; with
+ * Backward: dy / dn NULL: that output has no gradient.  du only where u was given, dz only where z was, dscale only where scale was, the
+ * gradients of a norm only where its gamma was given (else -1); any output may be NULL; with
  * u == NULL dx is the whole gradient of x.  dscale ... dpre_beta: [D] of type ptype, overwritten.  workspace: at least
  * mbvae_gated_norm_bwd_workspace(rows, D, dtype) bytes, 16-byte aligned.  Bitwise reproducible. */
 int mbvae_gated_norm_fwd(const void* x, int64_t ldx, const void* u, int64_t ldu, const void* z, int64_t ldz, const uint8_t* keep,

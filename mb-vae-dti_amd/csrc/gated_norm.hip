@@ -128,6 +128,7 @@ int mbvae_gated_norm_bwd(const void* x, int64_t ldx, const void* u, int64_t ldu,
   const int st = check(a, dtype, rows, D, ptype);
   if (st != MBVAE_OK) return st;
   if (lddy < 0 || lddn < 0 || (dn && !pre_gamma) || (rows && !stats) || !ws || ((uintptr_t)ws & 15)) return MBVAE_EINVAL;
+  if (dscale && !scale) return MBVAE_EINVAL;
   if ((dpost_gamma || dpost_beta) && !post_gamma) return MBVAE_EINVAL;
   if ((dpre_gamma || dpre_beta) && !pre_gamma) return MBVAE_EINVAL;
   if ((du && !u) || (dz && !z)) return MBVAE_EINVAL;

@@ -108,3 +108,18 @@ def test_gated_norm_entries_refuse_before_any_launch():
     assert bwd(ng=0) == EINVAL and bwd(pg=0, pb=0) == EINVAL and bwd(u=0) == EINVAL and bwd(z=0) == EINVAL
     assert bwd(stats=0) == EINVAL and bwd(lddn=-1) == EINVAL and bwd(ws=0) == EINVAL and bwd(ws=A + 8) == EINVAL
     assert bwd(ws_bytes=lib.mbvae_gated_norm_bwd_workspace(4, 8, 0) - 1) == EINVAL
+
+
+def test_gated_norm_backward_refuses_the_gradient_of_an_absent_vector():
+    """Each vector's gradient goes with the vector: nothing is summed for one that is not there, so its place would be filled with whatever the
+    workspace holds."""
+    lib = _lib.load()
+
+    def bwd(pg=A, scale=A, ng=A, dscale=0, dpg=0, dpb=0, dng=0, dnb=0, rows=4):
+        return lib.mbvae_gated_norm_bwd(A, 8, A, 8, A, 8, 0, 1.0, pg, 0, scale, ng, A, A, 8, 0, 8, A, A, A, dscale, dpg, dpb, dng, dnb, rows, 8, 0, 1e-5, 0, 0,
+                                        A, 1 << 20, 0)
+
+    for rows in (0, 4):
+        assert bwd(scale=0, dscale=A, rows=rows) == EINVAL
+        assert bwd(pg=0, dpg=A, rows=rows) == EINVAL and bwd(pg=0, dpb=A, rows=rows) == EINVAL
+        assert bwd(ng=0, dng=A, rows=rows) == EINVAL and bwd(ng=0, dnb=A, rows=rows) == EINVAL
