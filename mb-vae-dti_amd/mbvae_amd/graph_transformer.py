@@ -368,11 +368,13 @@ class GraphTransformer(nn.Module):
     def forward(self, X, E, y, node_mask, edge_ids=None):
         """edge_ids (optional, integers [bs,n,n]): the class of every pair whose row of E is one-hot, anything outside the classes
         (-1) where the row is all-zero.  The edge input MLP then runs once per class instead of once per pair; E itself is still
-        needed for the skip connection at the output."""
+        needed for the skip connection at the output, and may not ask for a gradient (it would get that of the skip connection alone)."""
         n = X.shape[1]
         if edge_ids is not None:
             if edge_ids.shape != E.shape[:-1] or edge_ids.is_floating_point() or edge_ids.dtype == torch.bool:
                 raise ValueError(f"edge_ids must be integers of shape {tuple(E.shape[:-1])}, got {edge_ids.dtype} {tuple(edge_ids.shape)}")
+            if torch.is_grad_enabled() and E.requires_grad:
+                raise ValueError("edge_ids: the gradient of E does not pass through a lookup; leave edge_ids out, or detach E")
             if edge_ids.dtype != torch.int64 and E.shape[-1] > torch.iinfo(edge_ids.dtype).max:
                 edge_ids = edge_ids.long()                       # (the all-zero row's id has to fit)
         X, E, y = X.float(), E.float(), y.float()

@@ -123,3 +123,18 @@ def test_gated_norm_backward_refuses_the_gradient_of_an_absent_vector():
         assert bwd(scale=0, dscale=A, rows=rows) == EINVAL
         assert bwd(pg=0, dpg=A, rows=rows) == EINVAL and bwd(pg=0, dpb=A, rows=rows) == EINVAL
         assert bwd(ng=0, dng=A, rows=rows) == EINVAL and bwd(ng=0, dnb=A, rows=rows) == EINVAL
+
+
+def test_denoiser_from_edge_classes_refuses_a_pair_gradient():
+    """With the classes at hand the edge input is looked up: E would get the skip connection's gradient and not its whole one."""
+    from mbvae_amd.graph_transformer import GraphTransformer
+    net = GraphTransformer(n_layers=1, input_dims={"X": 13, "E": 5, "y": 77}, hidden_mlp_dims={"X": 32, "E": 16, "y": 64},
+                           hidden_dims={"dx": 64, "de": 16, "dy": 64, "n_head": 4, "dim_ffX": 32, "dim_ffE": 16, "dim_ffy": 64},
+                           output_dims={"X": 5, "E": 5, "y": 64})
+    E = torch.zeros(2, 3, 3, 5, requires_grad=True)
+    args = torch.zeros(2, 3, 13), E, torch.zeros(2, 77), torch.ones(2, 3, dtype=torch.bool)
+    ids = torch.zeros(2, 3, 3, dtype=torch.int8)
+    with pytest.raises(ValueError, match="gradient of E"):
+        net(*args, edge_ids=ids)
+    with torch.no_grad(), pytest.raises(RuntimeError):          # (nothing to refuse without gradients: the kernels ask for a GPU next)
+        net(*args, edge_ids=ids)
