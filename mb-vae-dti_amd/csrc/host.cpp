@@ -317,6 +317,16 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(const Tensor& x, const OptTens
 }
 
 // ------------------------------------------------------------------------------------------------ gradient norm and clipping
+// Whether grad_clip takes these gradients (what it refuses with an error).
+bool grad_clip_takes(const std::vector<Tensor>& grads) {
+  const bool tangents = tangents_possible();
+  for (const Tensor& g : grads)
+    if (!g.is_cuda() || g.device() != grads[0].device() || g.layout() != at::kStrided || type_code(g.scalar_type()) < 0 || g.requires_grad() ||
+        !g.has_storage() || (tangents && g._fw_grad(0).defined()) || !(g.is_contiguous() || g.is_non_overlapping_and_dense()))
+      return false;
+  return true;
+}
+
 // max_norm < 0: the norm alone.  out empty: in place.
 Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, double max_norm, double p) {
   const char* what = "gradient norm";
@@ -366,4 +376,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding", &embedding);
   m.def("gated_residual_norm", &gated_residual_norm);
   m.def("grad_clip", &grad_clip);
+  m.def("grad_clip_takes", &grad_clip_takes);
 }

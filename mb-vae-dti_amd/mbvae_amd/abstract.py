@@ -141,17 +141,22 @@ class AbstractDTIModel(_Base):
     def configure_gradient_clipping(self, optimizer, gradient_clip_val=None, gradient_clip_algorithm=None):
         """Lightning's hook between backward and the optimiser step (Trainer(gradient_clip_val=...), mb_vae_dti/training/run.py:638-654):
         "norm" (the default) scales the gradients of the optimiser's parameters to a global 2-norm of at most gradient_clip_val and logs
-        the norm, "value" clamps every entry.  Nothing happens where gradient_clip_val is None or 0."""
-        if not gradient_clip_val:
+        the norm as train/grad_norm, "value" clamps every entry.  Nothing happens where gradient_clip_val is None, 0 or negative.  Gradients that
+        ops.clip_grad_norm_ does not take (float64, strided, on the host or on several devices) are clipped by torch."""
+        if gradient_clip_val is None or gradient_clip_val <= 0:
             return
-        params = [p for group in optimizer.param_groups for p in group["params"]]
-        if gradient_clip_algorithm in (None, "norm"):
-            norm = ops.clip_grad_norm_([p.grad for p in params], gradient_clip_val)
-            self.log("train/grad_norm", norm, on_step=False, on_epoch=True)
-        elif gradient_clip_algorithm == "value":
-            torch.nn.utils.clip_grad_value_(params, gradient_clip_val)
-        else:
+        if gradient_clip_algorithm not in (None, "norm", "value"):
             raise ValueError(f"gradient_clip_algorithm is 'norm' or 'value', got {gradient_clip_algorithm!r}")
+        params = [p for group in optimizer.param_groups for p in group["params"]]
+        if gradient_clip_algorithm == "value":
+            torch.nn.utils.clip_grad_value_(params, gradient_clip_val)
+            return
+        grads = [p.grad for p in params if p.grad is not None]
+        if grads and ops.clip_grad_norm_takes(grads):
+            norm = ops.clip_grad_norm_(grads, gradient_clip_val)
+        else:
+            norm = torch.nn.utils.clip_grad_norm_(params, gradient_clip_val)
+        self.log("train/grad_norm", norm, on_step=False, on_epoch=True)
 
     def setup_metrics(self, phase, finetune_score=None):
         """The reference fills the three slots with torchmetrics collections (modules/utils.py:180-222); those wrappers

@@ -1181,6 +1181,11 @@ def clip_grad_norm_(grads, max_norm, norm_type=2.0, out=None):
     return _lib.host().grad_clip(grads, outs or [], max_norm, norm_type)
 
 
+def clip_grad_norm_takes(grads):
+    """Whether clip_grad_norm_ takes these gradients: dense float32, bfloat16 or float16 tensors on one GPU that ask for no gradient themselves."""
+    return _lib.host().grad_clip_takes([g for g in grads if g is not None])
+
+
 # ------------------------------------------------------------------------------------------------ diffusion samplers
 @torch.no_grad()
 def apply_noise(X0, E0, node_mask, abar_t, mx, me, expX, expE):

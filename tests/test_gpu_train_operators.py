@@ -1068,3 +1068,32 @@ def test_embedding_forward_past_one_side_of_a_grid(ops):
         assert torch.equal(y[r:r + (1 << 20)], padded[ids[r:r + (1 << 20)].long() + 1]), f"rows from {r}"
     del y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind", ["kernels", "strided", "float64", "two places", "history"])
+def test_lightning_hook_by_kernels_and_by_torch(ops, kind):
+    """On the GPU the hook takes the kernels where they take the gradients and torch where they do not; the result is the same function."""
+    from mbvae_amd.abstract import AbstractDTIModel
+    g = _gen(80)
+    grads = [_randn(g, 40, 6).cuda(), _randn(g, 9).cuda(), _randn(g, 3, 4)[:, ::2].cuda()]
+    if kind == "strided":
+        grads.append(_randn(g, 50, 8).cuda()[:, ::2])
+    elif kind == "float64":
+        grads[1] = grads[1].double()
+    elif kind == "two places":
+        grads[0] = grads[0].cpu()
+    elif kind == "history":
+        grads[0] = grads[0].requires_grad_(True) * 1.0
+    model = AbstractDTIModel()
+    for i, t in enumerate(grads):
+        p = torch.nn.Parameter(torch.zeros(t.shape, dtype=t.dtype, device=t.device))
+        p.grad = t
+        model.register_parameter(f"p{i}", p)
+    model.register_parameter("unused", torch.nn.Parameter(torch.zeros(2, device="cuda")))
+    assert ops.clip_grad_norm_takes([p.grad for p in model.parameters()]) == (kind == "kernels")
+    want = [t.detach().double().cpu().clone() for t in grads]
+    norm = math.sqrt(sum(float(t.square().sum()) for t in want))
+    model.configure_gradient_clipping(torch.optim.SGD(model.parameters(), lr=0.1), 0.25 * norm)
+    for p, t in zip(model.parameters(), want):
+        check(p.grad, 0.25 * t, 0.25 * t.abs() * 16 * U, "clipped")        # (torch: an fp32 norm of a few hundred squares, a quotient, a product)
+    assert abs(float(model.logged["train/grad_norm"]) - norm) <= 16 * U * norm

@@ -138,3 +138,46 @@ def test_denoiser_from_edge_classes_refuses_a_pair_gradient():
         net(*args, edge_ids=ids)
     with torch.no_grad(), pytest.raises(RuntimeError):          # (nothing to refuse without gradients: the kernels ask for a GPU next)
         net(*args, edge_ids=ids)
+
+
+def _clipping_model(grads):
+    """A model whose parameters have the given gradients, and an optimiser over them."""
+    from mbvae_amd.abstract import AbstractDTIModel
+    model = AbstractDTIModel()
+    for i, g in enumerate(grads):
+        p = torch.nn.Parameter(torch.zeros(g.shape, dtype=g.dtype))
+        p.grad = g
+        model.register_parameter(f"p{i}", p)
+    return model, torch.optim.SGD(model.parameters(), lr=0.1)
+
+
+def _layouts():
+    g = torch.Generator().manual_seed(3)
+    a, b = torch.randn(40, 6, generator=g), torch.randn(9, generator=g)
+    return {"host": [a, b], "float64": [a.double(), b.double()], "mixed": [a, b.double()], "strided": [a[:, ::2], b],
+            "empty": [torch.zeros(0, 3), b], "with history": [a.clone().requires_grad_(True) * 1.0, b]}
+
+
+@pytest.mark.parametrize("kind", list(_layouts()))
+def test_lightning_hook_clips_what_the_kernels_do_not_take(kind):
+    """Gradients on the host, in float64, strided or with a history: clipped as Lightning's own hook does, by torch."""
+    grads = _layouts()[kind]
+    model, opt = _clipping_model(grads)
+    want = [t.detach().double().clone() for t in grads]
+    norm = math.sqrt(sum(float(t.square().sum()) for t in want))
+    model.configure_gradient_clipping(opt, 0.25 * norm)
+    for p, t in zip(model.parameters(), want):
+        assert torch.allclose(p.grad.detach().double(), 0.25 * t, rtol=1e-5, atol=1e-7)
+    assert float(model.logged["train/grad_norm"]) == pytest.approx(norm, rel=1e-5)
+
+
+def test_lightning_hook_without_anything_to_do():
+    """No limit, a limit of zero or below (Lightning clips for neither), and a model without gradients."""
+    model, opt = _clipping_model([torch.ones(4)])
+    for limit in (None, 0, 0.0, -1.0):
+        model.configure_gradient_clipping(opt, limit)
+        model.configure_gradient_clipping(opt, limit, "value")
+        assert bool((model.p0.grad == 1).all()) and "train/grad_norm" not in model.logged
+    model.p0.grad = None
+    model.configure_gradient_clipping(opt, 1.0)
+    assert float(model.logged["train/grad_norm"]) == 0
