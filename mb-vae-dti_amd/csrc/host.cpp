@@ -7,12 +7,14 @@
 #include <torch/csrc/autograd/forward_grad.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/DeviceGuard.h>
+#include <atomic>
 #include <cmath>
 #include <limits>
 #include <map>
 #include <string>
 
 typedef struct ihipStream_t* mbvae_stream_t;
+namespace py = pybind11;
 
 namespace {
 
@@ -36,7 +38,13 @@ struct Library {
   int (*grad_clip)(const void* const*, void* const*, const int64_t*, const int32_t*, int64_t, double, double, float*, void*, int64_t, mbvae_stream_t);
 } lib;
 
-void bind(const std::map<std::string, uintptr_t>& entries) {
+// While the package notes kernel calls (_lib.PROFILE), every call of an entry point is bracketed as its ctypes calls are: bracket(name) notes
+// the start and returns what notes the end.  Never freed: threads of autograd may outlast the interpreter.
+std::atomic<bool> profiling{false};
+py::object* bracket = nullptr;
+
+void bind(const std::map<std::string, uintptr_t>& entries, py::object noted) {
+  bracket = new py::object(std::move(noted));
 #define BIND(name) lib.name = reinterpret_cast<decltype(lib.name)>(entries.at("mbvae_" #name))
   BIND(gated_norm_fwd);
   BIND(gated_norm_bwd_workspace);
@@ -52,6 +60,21 @@ void bind(const std::map<std::string, uintptr_t>& entries) {
 void succeeded(int status, const char* entry) {
   TORCH_CHECK(status == 0, entry, " failed: ",
               status == -1 ? "invalid argument" : status == -2 ? "unsupported shape" : status == -3 ? "kernel launch failure" : "unknown status");
+}
+
+// Calls an entry point; raises on failure.
+template <typename F>
+void entry(const char* name, F call) {
+  if (!profiling.load(std::memory_order_relaxed)) return succeeded(call(), name);
+  const auto with_gil = [&](auto f) {                        // (autograd's threads do not hold it)
+    py::gil_scoped_acquire gil;
+    f();
+  };
+  PyObject* end = nullptr;
+  with_gil([&] { end = (*bracket)(name).release().ptr(); });
+  const int status = call();
+  with_gil([&] { py::reinterpret_steal<py::object>(end)(status); });
+  succeeded(status, name);
 }
 
 // ------------------------------------------------------------------------------------------------ operands
@@ -141,9 +164,10 @@ Tensor embedding_raw(const Tensor& ids, const Tensor& weight, double scale) {
   sizes.push_back(weight.size(1));
   Tensor y = at::empty(sizes, weight.options().requires_grad(false));
   const c10::DeviceGuard guard(weight.device());
-  succeeded(lib.embedding_fwd(ids.const_data_ptr(), id_code(ids.scalar_type()), weight.const_data_ptr(), y.mutable_data_ptr(), ids.numel(),
-                              weight.size(0), weight.size(1), (float)scale, type_code(weight.scalar_type()), stream_of(weight)),
-            "mbvae_embedding_fwd");
+  entry("mbvae_embedding_fwd", [&] {
+    return lib.embedding_fwd(ids.const_data_ptr(), id_code(ids.scalar_type()), weight.const_data_ptr(), y.mutable_data_ptr(), ids.numel(),
+                             weight.size(0), weight.size(1), (float)scale, type_code(weight.scalar_type()), stream_of(weight));
+  });
   return y;
 }
 
@@ -164,10 +188,11 @@ struct Embedding : torch::autograd::Function<Embedding> {
       const Rows d(dy, D);
       const c10::DeviceGuard guard(dy.device());
       const Tensor ws = bytes_on(dy, lib.embedding_bwd_workspace(rows, vocab, D, type_code(dy.scalar_type())));
-      succeeded(lib.embedding_bwd(ids.const_data_ptr(), id_code(ids.scalar_type()), d.t.const_data_ptr(), d.ld, dw.mutable_data_ptr(), rows, vocab, D,
-                                  (float)ctx->saved_data["scale"].toDouble(), type_code(dy.scalar_type()), ws.mutable_data_ptr(), ws.numel(),
-                                  stream_of(dy)),
-                "mbvae_embedding_bwd");
+      entry("mbvae_embedding_bwd", [&] {
+        return lib.embedding_bwd(ids.const_data_ptr(), id_code(ids.scalar_type()), d.t.const_data_ptr(), d.ld, dw.mutable_data_ptr(), rows, vocab, D,
+                                 (float)ctx->saved_data["scale"].toDouble(), type_code(dy.scalar_type()), ws.mutable_data_ptr(), ws.numel(),
+                                 stream_of(dy));
+      });
     }
     return differentiable_once({dw, Tensor(), Tensor()}, "embedding");
   }
@@ -208,10 +233,11 @@ std::tuple<Tensor, Tensor> gated_norm_raw(const Tensor& x, const Tensor& u, cons
   Tensor y = contiguous_like(x), n = pre_g.defined() ? contiguous_like(x) : Tensor();
   if (stats) *stats = stats_for(x, rows);
   const c10::DeviceGuard guard(x.device());
-  succeeded(lib.gated_norm_fwd(ptr(xr.t), xr.ld, ptr(ur.t), ur.ld, ptr(zr.t), zr.ld, (const uint8_t*)ptr(keep), (float)a.keep_scale, ptr(post_g),
+  entry("mbvae_gated_norm_fwd", [&] {
+    return lib.gated_norm_fwd(ptr(xr.t), xr.ld, ptr(ur.t), ur.ld, ptr(zr.t), zr.ld, (const uint8_t*)ptr(keep), (float)a.keep_scale, ptr(post_g),
                                ptr(post_b), ptr(scale), ptr(pre_g), ptr(pre_b), out_ptr(y), out_ptr(n), stats ? stats->data_ptr<float>() : nullptr, rows,
-                               D, a.rms, (float)a.eps, type_code(x.scalar_type()), param_code(post_g, scale, pre_g), stream_of(x)),
-            "mbvae_gated_norm_fwd");
+                               D, a.rms, (float)a.eps, type_code(x.scalar_type()), param_code(post_g, scale, pre_g), stream_of(x));
+  });
   return {y, n};
 }
 
@@ -258,13 +284,14 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     const int code = type_code(x.scalar_type());
     const c10::DeviceGuard guard(x.device());
     const Tensor ws = bytes_on(x, lib.gated_norm_bwd_workspace(rows, D, code));
-    succeeded(lib.gated_norm_bwd(ptr(xr.t), xr.ld, ptr(ur.t), ur.ld, ptr(zr.t), zr.ld, (const uint8_t*)ptr(keep),
+    entry("mbvae_gated_norm_bwd", [&] {
+      return lib.gated_norm_bwd(ptr(xr.t), xr.ld, ptr(ur.t), ur.ld, ptr(zr.t), zr.ld, (const uint8_t*)ptr(keep),
                                  (float)ctx->saved_data["keep_scale"].toDouble(), ptr(post_g), ptr(post_b), ptr(scale), ptr(pre_g),
                                  stats.data_ptr<float>(), ptr(dyr.t), dyr.ld, ptr(dnr.t), dnr.ld, out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]),
                                  out_ptr(out[5]), out_ptr(out[3]), out_ptr(out[4]), out_ptr(out[6]), out_ptr(out[7]), rows, D,
                                  ctx->saved_data["rms"].toBool(), (float)ctx->saved_data["eps"].toDouble(), code, param_code(post_g, scale, pre_g),
-                                 ws.mutable_data_ptr(), ws.numel(), stream_of(x)),
-              "mbvae_gated_norm_bwd");
+                                 ws.mutable_data_ptr(), ws.numel(), stream_of(x));
+    });
     return differentiable_once(std::move(out), "gated_residual_norm");
   }
 };
@@ -363,9 +390,10 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
   Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
   const Tensor ws = bytes_on(grads[0], lib.grad_clip_workspace((int64_t)count));
   const c10::DeviceGuard guard(device);
-  succeeded(lib.grad_clip(src.data(), write ? dst.data() : nullptr, numel.data(), types.data(), (int64_t)count, p, max_norm, norm.data_ptr<float>(),
-                          ws.mutable_data_ptr(), ws.numel(), stream_of(grads[0])),
-            "mbvae_grad_clip");
+  entry("mbvae_grad_clip", [&] {
+    return lib.grad_clip(src.data(), write ? dst.data() : nullptr, numel.data(), types.data(), (int64_t)count, p, max_norm, norm.data_ptr<float>(),
+                          ws.mutable_data_ptr(), ws.numel(), stream_of(grads[0]));
+  });
   return norm;
 }
 
@@ -373,6 +401,7 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind", &bind);
+  m.def("profile", [](bool on) { profiling = on; });
   m.def("embedding", &embedding);
   m.def("gated_residual_norm", &gated_residual_norm);
   m.def("grad_clip", &grad_clip);

@@ -5,6 +5,8 @@ entry point returns a non-zero status, a RuntimeError is raised.
 """
 import ctypes
 import os
+import sys
+import types
 from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -118,35 +120,66 @@ def host():
         except ImportError as e:
             raise RuntimeError(f"mbvae_amd/_host.so cannot be loaded ({e}): build it first (python mb-vae-dti_amd/build.py). "
                                "There is no fallback path.") from e
-        module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in SIGNATURES})
+        module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in SIGNATURES}, _bracket)
+        module.profile(_profile is not None)
         _host = module
     return _host
 
 
-# When set to a dict, every kernel call is bracketed by HIP events on the current torch stream:
-# PROFILE[(name, tag)] = [(start_event, end_event), ...]   (used by bench.py for per-kernel timings)
-PROFILE = None
+# PROFILE (below): the dict that kernel calls are noted in, or None
+_profile = None
+
+
+def _bracket(name, tag=None):
+    """Notes the start of a call of an entry point; the function it returns notes the end and takes the call's status."""
+    profile = _profile
+    if profile is None:
+        return lambda status: None
+    import torch
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+
+    def finish(status):
+        end.record()
+        if status == 0:
+            profile.setdefault((name, tag), []).append((start, end))
+    return finish
 
 
 def call(name, *args, tag=None, allow_unsupported=False):
     """Runs one entry point and raises on failure.  With allow_unsupported, an 'unsupported shape' status is not an
     error: the function returns False and the caller takes its other HIP route (never a CPU one)."""
     fn = getattr(load(), name)
-    if PROFILE is None:
+    if _profile is None:
         st = fn(*args)
     else:
-        import torch
-        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        start.record()
+        finish = _bracket(name, tag)
         st = fn(*args)
-        end.record()
-        if st == 0:
-            PROFILE.setdefault((name, tag), []).append((start, end))
+        finish(st)
     if st == -2 and allow_unsupported:
         return False
     if st != 0:
         raise RuntimeError(f"{name} failed: {_STATUS.get(st, st)}")
     return True
+
+
+class _Module(types.ModuleType):
+    """When PROFILE is set to a dict, every kernel call is bracketed by HIP events on the current torch stream:
+    PROFILE[(name, tag)] = [(start_event, end_event), ...]   (used by bench.py for per-kernel timings)"""
+
+    @property
+    def PROFILE(self):
+        return _profile
+
+    @PROFILE.setter
+    def PROFILE(self, profile):
+        global _profile
+        _profile = profile
+        if _host is not None:
+            _host.profile(profile is not None)
+
+
+sys.modules[__name__].__class__ = _Module
 
 
 class option:

@@ -1097,3 +1097,31 @@ def test_lightning_hook_by_kernels_and_by_torch(ops, kind):
     for p, t in zip(model.parameters(), want):
         check(p.grad, 0.25 * t, 0.25 * t.abs() * 16 * U, "clipped")        # (torch: an fp32 norm of a few hundred squares, a quotient, a product)
     assert abs(float(model.logged["train/grad_norm"]) - norm) <= 16 * U * norm
+
+
+def test_kernel_calls_are_noted_while_profiling(ops):
+    """_lib.PROFILE sees the calls of these operators as it sees all others, the backward's (issued from autograd's thread) among them, and
+    from the moment it is set on."""
+    from mbvae_amd import _lib
+    state = _training_state(90, rows=500)
+    plain = [t.clone() for t in _training_pass(ops, *state, 1.0)]
+    y = ops.embedding(state[0], state[1])
+    noted = {}
+    try:
+        _lib.PROFILE = noted
+        assert _lib.PROFILE is noted
+        y.sum().backward()
+        assert [k for k, _ in noted] == ["mbvae_embedding_bwd"]
+        got = _training_pass(ops, *state, 1.0)
+        ops.dense_from_ids(torch.zeros(1, 4, dtype=torch.int8, device="cuda"), torch.zeros(1, 4, 4, dtype=torch.int8, device="cuda"), 5, 5)
+        with pytest.raises(RuntimeError, match="invalid"):
+            ops.clip_grad_norm_([y.detach(), y.detach()], 1.0)
+    finally:
+        _lib.PROFILE = None
+    _training_pass(ops, *state, 1.0)
+    torch.cuda.synchronize()
+    assert {k: len(v) for (k, _), v in noted.items()} == {"mbvae_embedding_fwd": 1, "mbvae_embedding_bwd": 2, "mbvae_gated_norm_fwd": 1,
+                                                          "mbvae_gated_norm_bwd": 1, "mbvae_grad_clip": 1, "mbvae_dense_from_ids": 1}
+    assert all(0 < start.elapsed_time(end) < 1000 for calls in noted.values() for start, end in calls)
+    for a, b in zip(got, plain):
+        assert torch.equal(a, b)
