@@ -277,9 +277,10 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     }
     if (vectors) {
       const Tensor& any = post_g.defined() ? post_g : scale.defined() ? scale : pre_g;
-      const Tensor flat = at::empty({vectors * D}, any.options().requires_grad(false));
+      const int64_t piece = 16 / (int64_t)any.element_size(), step = (D + piece - 1) / piece * piece;      // (each begins at 16 bytes)
+      const Tensor flat = at::empty({vectors * step}, any.options().requires_grad(false));
       for (int i = 3, k = 0; i < 8; ++i)
-        if (wanted[i]) out[i] = part_of(flat, D * k++, D);
+        if (wanted[i]) out[i] = part_of(flat, step * k++, D);
     }
     const int code = type_code(x.scalar_type());
     const c10::DeviceGuard guard(x.device());

@@ -1125,3 +1125,21 @@ def test_kernel_calls_are_noted_while_profiling(ops):
     assert all(0 < start.elapsed_time(end) < 1000 for calls in noted.values() for start, end in calls)
     for a, b in zip(got, plain):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D", [1, 7, 64, 1037])
+@pytest.mark.parametrize("ptype", [F32, BF16, F16])
+def test_gradients_of_a_blocks_vectors_lie_apart_and_aligned(ops, D, ptype):
+    """They share one allocation: each begins at 16 bytes, ends where it ends, and writing one leaves the others."""
+    host = _block(_gen(D), (6, D), F32, ptype, True, False, False, True, True, True, "layer")
+    dev = {k: _device(v) if k not in ("keep_scale", "norm") else v for k, v in host.items()}
+    y, n = _call(ops, dev, 1e-5)
+    vectors = [dev["scale"], *dev["post"], *dev["pre"]]
+    (y.sum() + n.square().sum()).backward()
+    grads = [v.grad for v in vectors]
+    assert all(t.data_ptr() % 16 == 0 and t.is_contiguous() and t.shape == (D,) for t in grads)
+    before = [t.clone() for t in grads]
+    for i, t in enumerate(grads):
+        t.fill_(float(i))
+    assert all(bool((t == i).all()) for i, t in enumerate(grads)) and all(bool(torch.isfinite(t).all()) for t in before)
+    ops.clip_grad_norm_(grads, 0.5)                       # (refused if any two of them met)
