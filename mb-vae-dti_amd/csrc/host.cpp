@@ -386,8 +386,9 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
       dst[i] = o.mutable_data_ptr();
     }
   }
-  if (write)                                                 // (refused for tensors that may not be written here, so before the launch)
-    for (const Tensor& t : apart ? out : grads) t.unsafeGetTensorImpl()->bump_version();
+  if (write)
+    for (const Tensor& t : apart ? out : grads)
+      TORCH_CHECK(!t.is_inference() || c10::InferenceMode::is_enabled(), what, ": an inference tensor may not be written outside inference mode");
   Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
   const Tensor ws = bytes_on(grads[0], lib.grad_clip_workspace((int64_t)count));
   const c10::DeviceGuard guard(device);
@@ -395,6 +396,8 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
     return lib.grad_clip(src.data(), write ? dst.data() : nullptr, numel.data(), types.data(), (int64_t)count, p, max_norm, norm.data_ptr<float>(),
                           ws.mutable_data_ptr(), ws.numel(), stream_of(grads[0]));
   });
+  if (write)                                                 // (behind the call: one that is refused has written nothing)
+    for (const Tensor& t : apart ? out : grads) t.unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 

@@ -1143,3 +1143,27 @@ def test_gradients_of_a_blocks_vectors_lie_apart_and_aligned(ops, D, ptype):
         t.fill_(float(i))
     assert all(bool((t == i).all()) for i, t in enumerate(grads)) and all(bool(torch.isfinite(t).all()) for t in before)
     ops.clip_grad_norm_(grads, 0.5)                       # (refused if any two of them met)
+
+
+def test_clip_grad_norm_refused_leaves_no_trace(ops):
+    """A refused call has not written, and autograd is not told that it has: what was saved for a backward pass is still good."""
+    leaf = torch.ones(100, device="cuda", requires_grad=True)
+    a = torch.full((100,), 3.0, device="cuda")
+    y = leaf * a
+    for grads, kwargs in (([a, a], {}), ([a[:60], a[50:]], {}), ([a, torch.ones(100, device="cuda")], dict(out=[torch.ones(100, device="cuda"), a]))):
+        versions = a._version
+        with pytest.raises(RuntimeError, match="invalid"):
+            ops.clip_grad_norm_(grads, 1.0, **kwargs)
+        assert a._version == versions
+    y.sum().backward()
+    assert torch.equal(leaf.grad, a)
+    y = leaf * a
+    ops.clip_grad_norm_([a], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    with torch.inference_mode():
+        frozen = torch.full((100,), 3.0, device="cuda")
+        ops.clip_grad_norm_([frozen], 1.0)
+    assert float(frozen[0]) < 1
+    with pytest.raises(RuntimeError, match="nference"):
+        ops.clip_grad_norm_([torch.ones(100, device="cuda")], 1e-3, out=[frozen])
