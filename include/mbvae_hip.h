@@ -443,9 +443,10 @@ int mbvae_embedding_bwd(const void* ids, int id_type, const void* dy, int64_t ld
  *   norm = (sum |g|^p)^(1/p) over all values of all tensors (p = 1, 2 or infinity),   dst = src * min(1, max_norm / (norm + 1e-6)).
  * src, dst, numel, dtype are HOST arrays of `count` entries (device pointers, value counts, types 0 fp32 / 1 bf16 / 2 fp16), read
  * before the call returns; norm is one device float.  dst == NULL: the norm alone.  dst[i] == src[i] for all i: in place (nothing is
- * written where the norm is within max_norm).  An output may not share memory with another output, nor with an input other than
- * its own exact place: -1.  A norm of infinity scales by 0, a NaN norm makes every gradient NaN; a max_norm of infinity never
- * scales.  workspace: at least
+ * written where norm + 1e-6 <= max_norm; just above that, and for norms around 1e-6, values are scaled as the formula says).  An output
+ * may not share memory with another output, nor with an input other than its own exact place: -1.  The factor comes from the fp64 norm, of
+ * which *norm is the rounding: a finite norm beyond fp32 is returned as infinity and still scales by what it is.  Where a value is infinite the
+ * factor is 0, where one is NaN every gradient becomes NaN; a max_norm of infinity never scales.  workspace: at least
  * mbvae_grad_clip_workspace(count) bytes, 8-byte aligned.  Partial sums are fp64 in a fixed order: bitwise reproducible. */
 int64_t mbvae_grad_clip_workspace(int64_t count);
 int mbvae_grad_clip(const void* const* src, void* const* dst, const int64_t* numel, const int32_t* dtype, int64_t count, double p,

@@ -1163,8 +1163,9 @@ def global_grad_norm(grads, norm_type=2.0):
 def clip_grad_norm_(grads, max_norm, norm_type=2.0, out=None):
     """Scales a list of gradients (p.grad of a model's parameters; None entries are skipped) by min(1, max_norm / (norm + 1e-6)) and
     returns their norm before it as one float32 value on the GPU: what Lightning's gradient_clip_val does (mb_vae_dti/training/run.py:638-654).
-    In place, or into `out`: as many tensors of the same types and layouts.  float32, bfloat16 and float16 may be mixed.  Where the norm
-    is within max_norm, or max_norm is infinity, the values stay bit for bit; a norm of infinity scales by 0, a NaN norm makes every gradient
+    In place, or into `out`: as many tensors of the same types and layouts.  float32, bfloat16 and float16 may be mixed.  Where norm + 1e-6
+    <= max_norm, or max_norm is infinity, the values stay bit for bit.  The factor comes from the float64 norm: one beyond float32 is
+    returned as infinity and still scales by what it is.  Where a value is infinite the factor is 0, where one is NaN every gradient becomes
     NaN.  No tensor may share memory with another one that is written."""
     grads, outs = list(grads), None if out is None else list(out)
     if outs is not None and len(outs) != len(grads):

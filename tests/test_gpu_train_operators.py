@@ -1167,3 +1167,23 @@ def test_clip_grad_norm_refused_leaves_no_trace(ops):
     assert float(frozen[0]) < 1
     with pytest.raises(RuntimeError, match="nference"):
         ops.clip_grad_norm_([torch.ones(100, device="cuda")], 1e-3, out=[frozen])
+
+
+@pytest.mark.parametrize("size", [1e-9, 1e-7, 1e-3, 0.5, 3.0, 1e4])
+def test_clip_grad_norm_at_its_limit(ops, size):
+    """Limits on both sides of the norm: values stay bit for bit exactly where norm + 1e-6 <= max_norm, but for a factor that rounds to 1, and
+    follow the formula where the 1e-6 is all that there is (a norm of 1e-9 and a limit of 1e-7: a tenth)."""
+    g = _gen(95)
+    t = _randn(g, 5000)
+    t = t * (size / float(t.double().norm()))
+    norm = float(t.double().norm())
+    for max_norm in (norm, norm * (1 - 1e-3), norm * (1 + 1e-3), norm + 1e-6, math.nextafter(norm + 1e-6, math.inf), norm + 2e-6, 0.5 * norm, 1e-7, 1e-6):
+        _, _, want, bounds = clip_reference([t], max_norm, 2.0)
+        dev = t.cuda()
+        ops.clip_grad_norm_([dev], max_norm)
+        check(dev, want[0], bounds[0], f"limit {max_norm}")
+        factor = max_norm / (norm + 1e-6)
+        if factor >= 1 + 1e-12:                                        # (the norm's own last bits decide at 1)
+            assert torch.equal(dev.cpu(), t), f"limit {max_norm}: within the limit the values stay"
+        elif factor < 1 - 2 * U:
+            assert not torch.equal(dev.cpu(), t), f"limit {max_norm}: above the limit the values are scaled"
