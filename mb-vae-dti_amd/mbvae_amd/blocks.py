@@ -53,7 +53,10 @@ def _affine(ln):
 
 def _step(x, u, z, p, training, following):
     """(x + u * dropout(sigmoid(z)), LayerNorm `following` of it) in one kernel; u None: x itself is gated, z None: no gate.  Draws the
-    same keep mask as ops.gate_update."""
+    same keep mask as ops.gate_update.  Rows wider than the kernel holds take the separate ones."""
+    if x.shape[-1] > ops.GATED_NORM_MAX_WIDTH:
+        y = x + u if z is None else ops.gate_update(x, u, z, p, training)
+        return y, None if following is None else _ln(following, y)
     keep, scale = None, 1.0
     if z is not None and training and p > 0:
         keep = torch.empty(z.shape, dtype=torch.uint8, device=z.device).bernoulli_(1.0 - p)

@@ -377,6 +377,9 @@ def gate_update(x, u, z, drop_p=0.0, training=False):
 
 
 # ------------------------------------------------------------------------------------------------ gated residual norm
+GATED_NORM_MAX_WIDTH = 8192          # columns of a row that one block's registers hold
+
+
 def gated_residual_norm(x, u=None, z=None, keep=None, keep_scale=1.0, post=None, res_scale=None, pre=None, norm="layer", eps=1e-5):
     """What a residual block does around its products, in one kernel each way:
 

@@ -1187,3 +1187,21 @@ def test_clip_grad_norm_at_its_limit(ops, size):
             assert torch.equal(dev.cpu(), t), f"limit {max_norm}: within the limit the values stay"
         elif factor < 1 - 2 * U:
             assert not torch.equal(dev.cpu(), t), f"limit {max_norm}: above the limit the values are scaled"
+
+
+def test_fused_blocks_wider_than_the_kernel(ops):
+    """Hidden widths above 8192 run with the fused updates switched on as well: by the separate kernels, bit for bit."""
+    from mbvae_amd import blocks
+    torch.manual_seed(5)
+    for cls in (blocks.TransformerEncoder, blocks.ResidualEncoder):
+        net = cls(12, ops.GATED_NORM_MAX_WIDTH + 8, 4, 1, factor=1, dropout=0.1).cuda().train()
+        x = torch.randn(3, 12, device="cuda")
+        got = []
+        for fused in (False, True):
+            ops.set_fused_blocks(fused)
+            try:
+                torch.manual_seed(6)
+                got.append(net(x))
+            finally:
+                ops.set_fused_blocks(False)
+        assert torch.equal(got[0], got[1])
