@@ -136,14 +136,16 @@ void check_same(const Tensor& t, const Tensor& as, const char* what, const char*
   TORCH_CHECK_VALUE(t.device() == as.device(), what, ": ", name, ": expected a tensor on ", as.device(), ", got one on ", t.device());
 }
 
-// A tensor as rows of D contiguous elements: a view where the layout allows one, a copy otherwise.
+// A tensor as rows of D contiguous elements: a view where the layout allows one, a copy otherwise.  (The imaginary part of a conjugate
+// holds its values with the other sign and a mark, which kernels do not see.)
 struct Rows {
   Tensor t;
   int64_t ld = 0;
   Rows() {}
   Rows(const Tensor& x, int64_t D) {
     if (!x.defined()) return;
-    t = x.dim() == 2 ? x : x.reshape({-1, D});
+    t = x.resolve_neg();
+    if (t.dim() != 2) t = t.reshape({-1, D});
     if (D > 1 && t.size(0) > 0 && t.stride(1) != 1) t = t.contiguous();
     ld = t.size(0) > 1 ? t.stride(0) : D;
   }
@@ -206,7 +208,7 @@ Tensor embedding(const Tensor& ids, const Tensor& weight, double scale) {
   TORCH_CHECK_VALUE(weight.dim() == 2, "embedding: weight must be [V, D], got shape ", weight.sizes());
   TORCH_CHECK_VALUE(ids.numel() < ((int64_t)1 << 31) && weight.size(0) < ((int64_t)1 << 31) && weight.size(1) <= ((int64_t)1 << 23),
                     "embedding: at most 2^31 - 1 ids, 2^31 - 1 table rows and 2^23 columns");
-  const Tensor i = ids.contiguous(), w = weight.contiguous();
+  const Tensor i = ids.contiguous(), w = weight.resolve_neg().contiguous();
   if (at::GradMode::is_enabled() && w.requires_grad()) return Embedding::apply(w, i, scale);
   return embedding_raw(i, w, scale);
 }
@@ -326,7 +328,7 @@ std::tuple<Tensor, OptTensor> gated_residual_norm(const Tensor& x, const OptTens
     TORCH_CHECK_VALUE(t->device() == x.device(), what, ": ", name, ": expected a tensor on ", x.device(), ", got one on ", t->device());
     TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == D, what, ": ", name, " must have shape [", D, "], got ", t->sizes());
     first = &*t;
-    return t->contiguous();
+    return t->resolve_neg().contiguous();
   };
   const OptTensor pg = param(post_g, "post gamma"), pb = param(post_b, "post beta"), sc = param(scale, "res_scale"), ng = param(pre_g, "pre gamma"),
                   nb = param(pre_b, "pre beta");
@@ -382,6 +384,7 @@ Tensor grad_clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& ou
       TORCH_CHECK_VALUE(o.scalar_type() == g.scalar_type() && o.device() == device && o.sizes() == g.sizes() &&
                             (numel[i] <= 1 || o.strides() == g.strides()) && o.layout() == at::kStrided && !o.requires_grad(),
                         what, ": an output must have its gradient's type, shape, strides and device");
+      TORCH_CHECK_VALUE(o.is_neg() == g.is_neg(), what, ": an output must hold its values with the sign its gradient does");
       if (tangents) check_no_tangent(o, what);
       dst[i] = o.mutable_data_ptr();
     }

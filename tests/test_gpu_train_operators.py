@@ -1205,3 +1205,47 @@ def test_fused_blocks_wider_than_the_kernel(ops):
             finally:
                 ops.set_fused_blocks(False)
         assert torch.equal(got[0], got[1])
+
+
+def test_operands_that_are_marked_as_negated(ops):
+    """The imaginary part of a conjugate is a view of values with the other sign: every operand in turn against its materialised twin."""
+    g = _gen(100)
+
+    def marked(*shape):
+        t = torch.view_as_complex(_randn(g, *shape, 2).cuda()).conj().imag
+        assert t.is_neg()
+        return t
+
+    for D in (1, 6):
+        host = _block(g, (5, D), F32, F32, True, True, False, True, True, True, "layer")
+        plain = {k: _device(v, False) if k not in ("keep_scale", "norm") else v for k, v in host.items()}
+        for k in ("x", "u", "z", "scale", "post", "pre"):
+            shape = (5, D) if k in ("x", "u", "z") else (D,)
+            t = marked(*shape)
+            twin = t.clone().resolve_neg()
+            if k in ("post", "pre"):
+                pairs = [((t, plain[k][1]), (twin, plain[k][1])), ((plain[k][0], t), (plain[k][0], twin))]
+            else:
+                pairs = [(t, twin)]
+            for a, b in pairs:
+                for got, want in zip(_call(ops, {**plain, k: a}, 1e-5), _call(ops, {**plain, k: b}, 1e-5)):
+                    assert torch.equal(got, want), (k, D)
+        x = plain["x"].clone().requires_grad_(True)
+        y, n = _call(ops, {**plain, "x": x}, 1e-5)
+        dy = marked(5, D)
+        a, = torch.autograd.grad(y, x, dy, retain_graph=True)
+        b, = torch.autograd.grad(y, x, dy.clone().resolve_neg())
+        assert torch.equal(a, b)
+        ids, table = torch.tensor([0, 3, 3], device="cuda"), marked(4, D)
+        assert torch.equal(ops.embedding(ids, table), table.clone().resolve_neg()[ids])
+        w = plain["x"][:4].clone().requires_grad_(True)
+        y, dy = ops.embedding(ids, w), marked(3, D)
+        assert torch.equal(torch.autograd.grad(y, w, dy, retain_graph=True)[0], torch.autograd.grad(y, w, dy.clone().resolve_neg())[0])
+    t = torch._neg_view(torch.arange(1.0, 9.0, device="cuda"))
+    norm = ops.global_grad_norm([t])
+    check(norm, torch.tensor(204.0, dtype=torch.float64).sqrt(), 30 * U, "norm")
+    with pytest.raises(ValueError, match="sign"):
+        ops.clip_grad_norm_([t], 1.0, out=[torch.zeros(8, device="cuda")])
+    before = t.clone().resolve_neg()
+    ops.clip_grad_norm_([t], 0.5 * float(norm))
+    check(t, before.double() * 0.5, before.abs() * 8 * U, "clipped in place")
