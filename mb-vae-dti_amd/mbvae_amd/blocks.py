@@ -156,11 +156,13 @@ class AttentiveAggregator(nn.Module):
         self.projection = nn.Sequential(nn.LayerNorm(input_dim), nn.Linear(input_dim, output_dim), self.activation, nn.Dropout(dropout))
 
     def forward(self, features):
-        stacked = torch.stack(features, dim=-1)                                        # [B, D, V]
-        w = self.to_attn_logits.weight.reshape(1, -1, 1)
-        logits = (stacked * w).sum(1, keepdim=True) + self.to_attn_logits.bias.reshape(1, 1, 1)
-        attn = F.softmax(logits, dim=-1)                                               # [B, 1, V]
-        agg = (stacked * attn).sum(dim=-1)
+        # Views in the middle and the logits as one product: torch would sum over the columns of [B, D, V], and over all rows for the
+        # logits' weight, with several blocks an output, whose counters it clears by a memory-set node in a captured graph.
+        stacked = torch.stack(features, dim=1)                                         # [B, V, D]
+        rows = stacked.reshape(-1, stacked.shape[-1])
+        logits = ops.linear(rows, self.to_attn_logits.weight.reshape(1, -1), self.to_attn_logits.bias).reshape(stacked.shape[:2])
+        attn = F.softmax(logits, dim=-1).unsqueeze(1)                                  # [B, 1, V]
+        agg = (stacked * attn.transpose(1, 2)).sum(dim=1)
         h = _act_linear(self.projection[1], _ln(self.projection[0], agg), self.activation)
         return _drop(h, self.projection[3].p, self.training), attn
 
