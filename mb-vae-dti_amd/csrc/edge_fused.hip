@@ -1214,6 +1214,9 @@ __global__ __launch_bounds__(512) void edge_out_ln_fwd_kernel(EdgeOutArgs a) {
 
 static int ef_num_cus() { return mbvae_num_cus(); }
 
+// (A memory-set node of a captured graph has not cleared its memory on replays after the first; a kernel does.)
+static __global__ void clear_counter_kernel(int32_t* counter) { *counter = 0; }
+
 extern "C" {
 
 // E [bs,n,n,de] dense, W12 [2dx,de] (rows 0..dx-1: e_mul, dx..2dx-1: e_add), b12 [2dx] or null; Q,K,V [bs,n,dx]
@@ -1253,8 +1256,8 @@ static int edge_fused_fwd_impl(const float* E, const float* W12, const float* b1
     // dynamic order: about four tasks per workgroup are enough to even out a ragged batch
     ichunks = 1;
     while (ichunks < 8 && 2 * ichunks <= n && bs * ichunks < 4 * (int64_t)cus) ichunks *= 2;
-    if (((uintptr_t)work_counter & 3) || hipMemsetAsync(work_counter, 0, sizeof(int32_t), stream) != hipSuccess)
-      return MBVAE_EINVAL;
+    if ((uintptr_t)work_counter & 3) return MBVAE_EINVAL;
+    hipLaunchKernelGGL(clear_counter_kernel, dim3(1), dim3(1), 0, stream, work_counter);
   }
   EdgeFusedArgs a{E, W12, b12, Q, K, V, (int)ldq, ye_add, ye_mul, mask, P, wV, lse, E12, (int)bs, (int)n, scale, ichunks,
                   work_counter, node_off, graph_order, 1};

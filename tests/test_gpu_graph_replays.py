@@ -116,3 +116,38 @@ def test_encoder_train_step_with_adam_replays(tmp_path, fused):
     for k, (a, b) in enumerate(zip(*losses)):
         assert abs(a - b) <= 1e-3 * abs(a), f"step {k}: {losses}"
     assert losses[0][-1] < 0.9 * losses[0][0]
+
+
+@pytest.mark.parametrize("bs,low,high", [(3, 4, 20), (64, 10, 65), (300, 30, 65)])
+def test_denoiser_inference_replays(tmp_path, bs, low, high):
+    """The denoiser at its full widths over a ragged batch without gradients (the reverse step's network): the fused edge kernel takes its tasks
+    from a counter that every call has to clear, also in a replay behind calls that have used it up."""
+    from mbvae_amd.graph_transformer import GraphTransformer
+    from mbvae_amd.trainstep import CFG3, synthetic_graphs
+    torch.manual_seed(bs)
+    net = GraphTransformer(**{**CFG3, "n_layers": 2}).cuda().eval()
+    g = torch.Generator().manual_seed(bs)
+    sizes = torch.randint(low, high, (bs,), generator=g)
+    X0, E, mask = synthetic_graphs(bs, int(sizes.max()), "cuda", g, sizes=sizes)
+    X = torch.cat((X0, torch.randn(bs, X0.shape[1], CFG3["input_dims"]["X"] - X0.shape[2], generator=g).cuda()), 2)
+    y = torch.randn(bs, CFG3["input_dims"]["y"], generator=g).cuda()
+    with torch.no_grad():
+        net.prepare_padding_shortcuts(mask)
+
+        def step():
+            out = net(X, E, y, mask)
+            return [out.X, out.E, out.y]
+
+        graph, captured, nodes = _capture(step, tmp_path)
+        assert nodes["MEMSET"] == 0, nodes
+        for turn in range(4):
+            X.mul_(0.9)
+            y.neg_()
+            want = [t.clone() for t in step()]
+            for t in captured:
+                t.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for k, a, b in zip("XEy", captured, want):
+                assert torch.equal(a, b), f"replay {turn}, {k}"
