@@ -137,7 +137,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void embedding_few_join_kernel(const float* __restrict__ part, T* __restrict__ dW, int blocks, int64_t values, float scale) {
   __shared__ float red[32][9];
   const int cx = threadIdx.x & 7, g = threadIdx.x >> 3;
-  const int64_t c = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * 8 + cx;
+  const int64_t c = (int64_t)blockIdx.x * 8 + cx;
   float a[8] = {};
   if (c < values) {
     int b = g;
@@ -556,10 +556,16 @@ int chunk_for(int64_t rows, int64_t D) {
 // Blocks that clear `values` elements.
 int64_t clear_blocks(int64_t values) { return std::min<int64_t>(std::max<int64_t>(1, values / (4 * SORT_THREADS * 4)), 512); }
 
-// The route (see the top): few classes while their cells fit LDS, few tokens while the list of one block does.
+// The route (see the top): few tokens while the list of one block fits LDS; few classes while their cells do and the blocks' tables stay small
+// next to what an ordering costs.  Near FEW_CELLS a block adds up no more rows than its table has, so that many blocks of wide tables would
+// write, and read again, as much as dy holds.  Few classes / ordered, us, fp32: 16 384 rows of 5 x 512 16.5 / 30.4, 5 x 1024 25 / 37,
+// 8 x 1024 34 / 34, 12 x 512 29 / 25, 32 x 128 17 / 20, 32 x 512 85 / 24; 4096 rows of 5 x 4096 25 / 31, 8 x 4096 34 / 33, 32 x 256 22 / 18;
+// 131 072 of 5 x 1024 156 / 174, 16 x 512 110 / 97; bf16: 16 384 rows of 16 x 256 17 / 23, 8 x 512 22 / 27, 12 x 512 38 / 26, 131 072 of
+// 8 x 512 58 / 77, 12 x 512 108 / 74.  One or two classes are never worth an order: 16 384 rows of 2 x 4096 67 / 91 and 46 / 72.
 enum Route { FEW_CLASSES, FEW_TOKENS, RADIX_SORT };
 constexpr int64_t FEW_CELLS = 128;              // columns a thread x classes: 128 KB of LDS
 constexpr int64_t FEW_BLOCKS = 1024;
+constexpr int64_t FEW_PARTIALS = 5120 * 512;    // values in the tables of the first 512 blocks (more blocks have rows enough each)
 template <typename T>
 constexpr int vec() { return MbvaeVec<T>::N; }
 int vec_of(int dtype) { return dtype == MBVAE_F32 ? vec<float>() : vec<mbvae_bf16>(); }
@@ -575,10 +581,11 @@ Plan plan_for(int64_t rows, int64_t V, int64_t D, int dtype) {
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   p.lanes = lanes_for((D + vec_of(dtype) - 1) / vec_of(dtype), 64);
-  p.route = V * vec_of(dtype) <= FEW_CELLS ? FEW_CLASSES : rows <= ORDER_TOKENS && V < ORDER_VOCAB ? FEW_TOKENS : RADIX_SORT;
+  const int64_t teams = 256 / p.lanes, few_blocks = std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS, (rows + 8 * teams - 1) / (8 * teams)));
+  if (V * vec_of(dtype) <= FEW_CELLS && (V <= 2 || V * D * std::min<int64_t>(few_blocks, 512) <= FEW_PARTIALS)) p.route = FEW_CLASSES;
+  else p.route = rows <= ORDER_TOKENS && V < ORDER_VOCAB ? FEW_TOKENS : RADIX_SORT;
   if (p.route == FEW_CLASSES) {
-    const int64_t teams = 256 / p.lanes;
-    p.blocks = std::max<int64_t>(1, std::min<int64_t>(FEW_BLOCKS, (rows + 8 * teams - 1) / (8 * teams)));
+    p.blocks = few_blocks;
     p.part = take(4 * p.blocks * V * D);
   } else {
     p.chunk = chunk_for(rows, D);
@@ -641,7 +648,7 @@ int launch_bwd(const Plan& p, const void* ids, int id_type, const T* dy, int64_t
     if (!MBVAE_ALLOW_BIG_LDS(embedding_few_kernel<T>)) return MBVAE_ELAUNCH;
     hipLaunchKernelGGL((embedding_few_kernel<T>), dim3((unsigned)p.blocks, (unsigned)((D + width - 1) / width)), dim3(256), V * vec<T>() * 1024, stream,
                        ids, id_type, dy, ldy, part, rows, (uint32_t)V, D, p.lanes);
-    hipLaunchKernelGGL((embedding_few_join_kernel<T>), grid_of((values + 7) / 8), dim3(256), 0, stream, part, dW, (int)p.blocks, values, scale);
+    hipLaunchKernelGGL((embedding_few_join_kernel<T>), dim3((unsigned)((values + 7) / 8)), dim3(256), 0, stream, part, dW, (int)p.blocks, values, scale);
     return mbvae_launch_status();
   }
   if (p.route == FEW_TOKENS) {

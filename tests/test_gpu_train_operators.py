@@ -1043,7 +1043,7 @@ def test_clip_grad_norm_by_a_factor_below_fp32(ops, dtype, value, max_norm, p):
 
 @pytest.mark.parametrize("V,dtype", [(16, F32), (16, BF16), (40, F16)])
 def test_embedding_of_the_widest_rows(ops, V, dtype):
-    """Rows of 2^23 values.  With 16 classes the join of the blocks' tables has 2^27 values, more than one side of a grid holds; 40 are ordered."""
+    """Rows of 2^23 values: few classes and many."""
     D = 1 << 23
     dy = torch.randn(3, D, device="cuda").to(dtype)
     ids = torch.tensor([0, V - 1, V - 1], device="cuda")
@@ -1249,3 +1249,33 @@ def test_operands_that_are_marked_as_negated(ops):
     before = t.clone().resolve_neg()
     ops.clip_grad_norm_([t], 0.5 * float(norm))
     check(t, before.double() * 0.5, before.abs() * 8 * U, "clipped in place")
+
+
+@pytest.mark.parametrize("rows,V,D,dtype", [(16384, 5, 1024, F32), (16384, 5, 1025, F32), (16353, 5, 1025, F32), (40000, 5, 1024, BF16), (40000, 5, 1028, BF16),
+                                            (32768, 32, 160, F32), (32768, 32, 161, F32), (33000, 16, 512, BF16), (4096, 32, 640, F32), (4096, 32, 641, F32),
+                                            (100, 32, 20000, F32), (8, 1, 1 << 20, F16), (3, 2, (1 << 21) - 1, F32), (16384, 2, 4096, BF16),
+                                            (16384, 3, 4096, BF16)])
+def test_embedding_gradient_where_the_routes_meet(ops, rows, V, D, dtype):
+    """Few classes on both sides of the table size from which they are ordered.  A workspace is never as large as dy but for the smallest."""
+    from mbvae_amd import _lib
+    g = _gen(rows + D)
+    ids, dy = _ids(g, rows, V, "hot", torch.int8), _randn(g, rows, D, dtype=dtype)
+    weight = torch.zeros(V, D, dtype=dtype, device="cuda", requires_grad=True)
+    y = ops.embedding(ids.cuda(), weight, 0.5)
+    dw, = torch.autograd.grad(y, weight, dy.cuda(), retain_graph=True)
+    check(dw, *embedding_gradient(ids, dy, V, 0.5), "dweight")
+    assert torch.equal(torch.autograd.grad(y, weight, dy.cuda())[0], dw)
+    size = rows * D * dy.element_size()
+    code = {F32: 0, BF16: 1, F16: 2}[dtype]
+    assert _lib.query("mbvae_embedding_bwd_workspace", rows, V, D, code) <= max(22 << 20, size // 2)
+
+
+def test_embedding_gradient_workspace_stays_small(ops):
+    """Many rows of few, wide classes: the blocks' tables are bounded, whatever the rows."""
+    from mbvae_amd import _lib
+    for code, most in ((0, 32), (1, 16), (2, 16)):
+        for rows in (1000, 32768, 1 << 20, (1 << 31) - 1):
+            for V in (1, 5, most):
+                for D in (64, 512, 5120, 65536, 1 << 23):
+                    dy = rows * D * (4 if code == 0 else 2)
+                    assert _lib.query("mbvae_embedding_bwd_workspace", rows, V, D, code) <= max(22 << 20, dy // 3 + 20 * rows), (code, rows, V, D)
