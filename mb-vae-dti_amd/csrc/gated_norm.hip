@@ -11,9 +11,10 @@
 // reads anyway) instead of being read.  The column sums are kept in registers over all rows of a team, joined per block, and the blocks'
 // partials are added by a second kernel in a fixed order: reproducible, no atomics.
 // All sums, statistics and intermediate values are fp32; outputs are rounded once.
-// Measured (us; rate over what has to be read and written): 1 M rows of 64 fp32 values with a gate, forward 247 (4.3 TB/s), backward 388
+// Measured (us; rate over what each kernel reads and writes): 1 M rows of 64 fp32 values with a gate, forward 247 (5.4 TB/s), backward 388
 // (5.5 TB/s); 16 384 rows of 256 bf16 values with both norms, gate and scale 13.4 and 21.2 (3.1 and 3.2 TB/s); 4095 rows of 1037 fp16
-// values, root-mean-square norms, 17.6 and 34.8; 256 rows of 512 fp32 values 5.0 and 6.5 (a launch); the column sums' join 3-6.
+// values, root-mean-square norms, 17.6 and 35 (1.9 and 1.5 TB/s); 4096 rows of 8192 fp32 values with everything 252 and 925 (2.7 and 1.2 TB/s:
+// 1024 threads leave 128 registers, and both spill); 256 rows of 512 fp32 values 5.0 and 6.6 (a launch); the column sums' join 3-6.
 #include "gated_norm.h"
 #include <algorithm>
 

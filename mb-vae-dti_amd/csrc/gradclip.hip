@@ -7,9 +7,9 @@
 // its share backwards, so that it begins with what the norm has read last and what may still be in the last-level cache.
 // The tensor table travels in the kernel arguments, so that a call can be captured into a graph and needs no staging buffer: in those of
 // both kernels where it fits (TENSORS), otherwise in those of small kernels that put it together in the workspace.
-// Measured: 73 M fp32 values in 472 tensors 89 + 97 us, 302 M bf16 values in nine 143 + 214 us, both 4.7-5.1 TB/s over the two reads and
-// the write (a large copy: 4.7-5.4).  512 or 2048 blocks, 2 or 8 accesses a thread, and chunks dealt out in turn instead of
-// contiguous shares were all within 5 %: what is left is the second read.
+// Measured: 73 M fp32 values in 472 tensors 89 (3.3 TB/s) + 97 us (6.0 TB/s, in part from the last-level cache) behind three table launches of
+// 2-5 us; 302 M bf16 values in nine tensors 142 (4.2 TB/s) + 215 us (5.6 TB/s).  A large copy: 4.7-5.4 TB/s.  512 or 2048 blocks, 2 or 8
+// accesses a thread, and chunks dealt out in turn instead of contiguous shares were all within 5 %.
 #include "typed.h"
 #include <algorithm>
 #include <cmath>
