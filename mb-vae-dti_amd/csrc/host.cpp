@@ -352,7 +352,7 @@ bool grad_clip_takes(const std::vector<Tensor>& grads) {
   const bool tangents = tangents_possible();
   for (const Tensor& g : grads)
     if (!g.is_cuda() || g.device() != grads[0].device() || g.layout() != at::kStrided || type_code(g.scalar_type()) < 0 || g.requires_grad() ||
-        !g.has_storage() || (tangents && g._fw_grad(0).defined()) || !(g.is_contiguous() || g.is_non_overlapping_and_dense()))
+        !g.has_storage() || g.unsafeGetTensorImpl()->is_python_dispatch() || (tangents && g._fw_grad(0).defined()) || !(g.is_contiguous() || g.is_non_overlapping_and_dense()))
       return false;
   return true;
 }

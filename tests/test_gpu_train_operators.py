@@ -1279,3 +1279,18 @@ def test_embedding_gradient_workspace_stays_small(ops):
                 for D in (64, 512, 5120, 65536, 1 << 23):
                     dy = rows * D * (4 if code == 0 else 2)
                     assert _lib.query("mbvae_embedding_bwd_workspace", rows, V, D, code) <= max(22 << 20, dy // 3 + 20 * rows), (code, rows, V, D)
+
+
+def test_clip_grad_norm_leaves_tensor_subclasses_to_torch(ops):
+    """Gradients that only look like tensors in memory (a distributed tensor is one) are not the kernels' to take."""
+    class Wrapped(torch.Tensor):
+        @staticmethod
+        def __new__(cls, inner):
+            return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device, strides=inner.stride())
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError(str(func))
+
+    plain = torch.ones(8, device="cuda")
+    assert ops.clip_grad_norm_takes([plain]) and not ops.clip_grad_norm_takes([plain, Wrapped(plain)])
